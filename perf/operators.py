@@ -159,8 +159,7 @@ def prepare(case, seed):
         st["parent"] = torch.tensor(_parents(case), device=dev, dtype=torch.int32)
         st["record"] = torch.empty((T * _record_row(case),), device=dev)
     if case["what"] == "commit":
-        st["parent"] = torch.tensor(_parents(case), device=dev, dtype=torch.int32)
-        st["record"] = torch.stack([_pending(case, st["off"], st["parent"], randn, rand) for _ in range(L)])
+        st["record"] = torch.stack([_pending(case, randn, rand) for _ in range(L)])
         st["state"] = 0.1 * randn(L, n, hv, dv, dk)
         st["state_out"] = torch.empty_like(st["state"])
         st["ring"] = randn(L, n, RING, C).to(dt)
@@ -176,7 +175,7 @@ def prepare(case, seed):
 
 
 def _record_row(c):
-    """f32 values that a verify pass leaves of a row: u of every value head, the unit k of every key head, the decay along its path."""
+    """f32 values that a verify pass leaves of a row: u of every value head, the unit k of every key head, its decays."""
     return c["v_heads"] * c["v_dim"] + c["k_heads"] * c["k_dim"] + c["v_heads"]
 
 
@@ -188,17 +187,11 @@ def _record_parts(c, record):
             record[..., a + b:].reshape(*record.shape[:-1], T, c["v_heads"]))
 
 
-def _pending(c, off, parent, randn, rand):
+def _pending(c, randn, rand):
     """A record as a verify pass leaves it."""
     T, hv, hk = sum(_lengths(c)), c["v_heads"], c["k_heads"]
     k = randn(T, hk, c["k_dim"])
-    step = -0.3 * rand(T, hv)
-    first = off[:-1].repeat_interleave(off[1:] - off[:-1])
-    decay, at = step.clone(), parent.long()
-    for _ in range(16):          # a root path has sixteen rows at most
-        decay = decay + step[(first + at).clamp(min=0)] * (at >= 0)[:, None]
-        at = torch.where(at >= 0, parent[(first + at).clamp(min=0)].long(), at)
-    return torch.cat([0.5 * randn(T * hv * c["v_dim"]), (k / k.norm(dim=-1, keepdim=True)).reshape(-1), decay.reshape(-1)])
+    return torch.cat([0.5 * randn(T * hv * c["v_dim"]), (k / k.norm(dim=-1, keepdim=True)).reshape(-1), -0.3 * rand(T * hv)])
 
 
 def _results(paths, base):
@@ -221,7 +214,7 @@ def _plan(st):
     at = lambda k: st[k].data_ptr() if k in st else None  # noqa: E731
     st["layer"] = ts.GatedDelta(c["k_heads"], c["v_heads"], c["k_dim"], c["v_dim"], c["taps"], ts.BF16 if c["dtype"] == "bf16" else ts.F16,
                                 conv=at("conv"), a_log=at("a_log"), dt_bias=at("dt_bias"), norm=at("norm"), l2_eps=L2_EPS, norm_eps=NORM_EPS)
-    st["batch"] = st["layer"].batch(st["offsets"], at("base"), at("parent") if c["tree"] else None)
+    st["batch"] = st["layer"].batch(st["offsets"], at("base"), at("parent") if c["what"] == "step" and c["tree"] else None)
     gate = dict(z=at("z"), z_stride=st["z"].stride(0)) if "z" in st and c["gated"] else {}
     if c["what"] == "conv":
         st["io"] = ts.GdnConv(qkv=at("qkv"), qkv_stride=st["qkv"].stride(0), a=at("a"), b=at("b"), gate_stride=st["a"].stride(0),
@@ -431,18 +424,19 @@ def _plain_step(st):
         w = torch.exp((Gl - G).masked_fill(~real[:, None], -math.inf)).float()
         state = torch.exp(Gl).float()[..., None] * S + (u * w[..., None]).transpose(-1, -2) @ k
         return dict(out=out, ring=ring, state=state)
-    parts = (u.transpose(1, 2)[real], k1[real], G.float().transpose(1, 2)[real])
+    parts = (u.transpose(1, 2)[real], k1[real], g)
     return dict(out=out, ring=ring, record=torch.cat([p.reshape(-1) for p in parts]))
 
 
 def _plain_commit(st):
     c, off, base, L = st["case"], st["off"], st["base"], st["case"]["layers"]
-    u, k, G = _record_parts(c, st["record"])
+    u, k, g = _record_parts(c, st["record"])
     rep = c["v_heads"] // c["k_heads"]
     path, keep = st["path"], st["keep"]
     on = torch.arange(16, device=off.device) < keep[:, None]
     rows = off[:-1, None] + path[:, :16]
-    u, k, G = u[:, rows], k[:, rows], G[:, rows]                           # layers x sequences x 16 x ..
+    u, k = u[:, rows], k[:, rows]                                          # layers x sequences x 16 x ..
+    G = (g[:, rows] * on[:, :, None]).cumsum(2)
     end = G.gather(2, (keep - 1)[None, :, None, None].expand(L, -1, 1, c["v_heads"]))
     w = torch.exp(end - G) * on[:, :, None]
     S = st["state"] * (base > 0)[:, None, None, None]
@@ -543,41 +537,38 @@ def _exact_prefill(st):
 def _exact_step(st):
     c = st["case"]
     rep = c["v_heads"] // c["k_heads"]
-    out, us, ks, Gs, ends = [], [], [], [], []
+    out, us, ks, gs, ends = [], [], [], [], []
     parents = _parents(c)
     for s, n in enumerate(_lengths(c)):
         parent = parents[st["offsets"][s]:st["offsets"][s + 1]]
         q, k, v, g, beta = _exact_convolved(st, s, parent)
         root = st["state"][s].double() * (1.0 if c["base"] > 0 else 0.0)
-        states, decay = {-1: root}, {-1: torch.zeros_like(g[0])}
+        states = {-1: root}
         for i in range(n):
             states[i], u, o = _exact_row(c, states[parent[i]], q[i].repeat_interleave(rep, 0), k[i].repeat_interleave(rep, 0), v[i], g[i], beta[i])
-            decay[i] = decay[parent[i]] + g[i]
             out.append(o)
             us.append(u)
-            Gs.append(decay[i])
         ks.append(k)
+        gs.append(g)
         ends.append(states[n - 1])
     o, ring = _exact_gate(st, torch.stack(out)), _exact_ring(st, 16)
     if c["final"]:
         return dict(out=o, ring=ring, state=torch.stack(ends))
-    return dict(out=o, ring=ring, record=torch.cat([torch.stack(us).reshape(-1), torch.cat(ks).reshape(-1), torch.stack(Gs).reshape(-1)]))
+    return dict(out=o, ring=ring, record=torch.cat([torch.stack(us).reshape(-1), torch.cat(ks).reshape(-1), torch.cat(gs).reshape(-1)]))
 
 
 def _exact_commit(st):
     c, L = st["case"], st["case"]["layers"]
     rep = c["v_heads"] // c["k_heads"]
-    u, k, G = _record_parts(c, st["record"].double())
+    u, k, g = _record_parts(c, st["record"].double())
     ring, S = st["ring_before"].double(), st["state"].double()
     if c["base"] == 0:
         S = torch.zeros_like(S)
     for s, path in enumerate(_paths(c)):
-        before = torch.zeros(L, c["v_heads"], device=S.device, dtype=torch.float64)
         slots = ring[:, s].clone()
         for i, p in enumerate(path):
             r = st["offsets"][s] + p
-            S[:, s] = torch.exp(G[:, r] - before)[..., None, None] * S[:, s] + u[:, r][..., None] * k[:, r].repeat_interleave(rep, 1)[..., None, :]
-            before = G[:, r]
+            S[:, s] = torch.exp(g[:, r])[..., None, None] * S[:, s] + u[:, r][..., None] * k[:, r].repeat_interleave(rep, 1)[..., None, :]
             ring[:, s, (c["base"] + i) % RING] = slots[:, (c["base"] + p) % RING]
     return dict(ring=ring, state=S)
 
