@@ -447,6 +447,129 @@ const uint16_t* tsv_device_logits(tsv_ctx* ctx);
 int64_t tsv_max_context(const tsv_ctx* ctx);
 int64_t tsv_vocab(const tsv_ctx* ctx);
 
+/* ---- recurrent layers: the mixer of a gated-delta-rule layer ---------------------------------
+ * What a host that verifies drafts for a hybrid target runs in its recurrent layers, beside the attention layers a handle
+ * serves (the reference's one batched verify forward is of such a family: crates/runtime/src/families/qwen/batched.rs:92-456,
+ * its state folded by rollback_retaining / commit_pending, real_forward_rollback.rs:268-435,501-530).  There is no handle:
+ * like tsv_accept_greedy_noalloc these calls take the caller's DEVICE memory and stream, allocate nothing, copy nothing from
+ * the host, wait for nothing and can be captured into a HIP graph (a stream of the caller's own; that of the current device).
+ *
+ * One head keeps a state S (k_dim x v_dim); a row with unit vectors q, k, a value row v, a decay g <= 0 and beta takes it to
+ *     S' = e^g S,   u = beta (v - S'^T k),   S_new = S' + k u^T,   o = scale S_new^T q.
+ * Value head h reads q and k of head h / (n_v_heads / n_k_heads).  q, k, v come from a projection's row of `channels` =
+ * 2 n_k_heads k_dim + n_v_heads v_dim values (q heads, k heads, v heads) through a causal depthwise convolution of conv_width
+ * taps (the last tap is the row itself) and SiLU; q and k are then divided by sqrt(sum of squares + l2_eps);
+ * g = -exp(a_log) softplus(a + dt_bias), beta = sigmoid(b).  With z the result of a head becomes
+ *     o / sqrt(mean(o^2) + norm_eps) * norm * silu(z).
+ *
+ * States: f32, n_seq x n_v_heads x v_dim x k_dim (one run of k_dim per value channel), 16-byte aligned.  The convolution's
+ * state is a ring of TSV_GDN_RING raw projection rows a sequence (n_seq x TSV_GDN_RING x channels, the rows' type): position p
+ * lies in slot p % TSV_GDN_RING, so that nothing has to be erased when a pass is rejected.  A sequence whose base is 0 starts
+ * from nothing, whatever its state and ring hold.
+ *
+ * Rows are bf16 or fp16.  Strides are elements from row to row, multiples of 8; qkv, q, k, v, z, out and the rings are 16-byte
+ * aligned.  Rows outside the batch's sequences are neither read nor written.  Outputs must not overlap inputs, but for state_out
+ * == state_in and ring_out == ring_in. */
+#define TSV_GDN_RING 32     /* raw rows kept per sequence: conv_width - 1 behind a pass and TSV_MAX_ROWS of it */
+#define TSV_GDN_MAX_SEQ 256 /* sequences of one call */
+typedef struct {
+    int32_t n_k_heads, n_v_heads; /* n_v_heads a multiple of n_k_heads */
+    int32_t k_dim, v_dim;         /* k_dim 64, 128 or 256; v_dim a multiple of 16, 16..256 */
+    int32_t conv_width;           /* taps, 1..4 */
+    int32_t dtype;                /* TSV_BF16 or TSV_F16: every row below */
+    float scale;                  /* <= 0: 1 / sqrt(k_dim) */
+    float l2_eps, norm_eps;
+    /* device, f32: channels x conv_width; n_v_heads; n_v_heads; v_dim (NULL where the call does not need it) */
+    const float *conv, *a_log, *dt_bias, *norm;
+} tsv_gdn_layer;
+/* The rows of a call: sequence s owns rows [offsets[s], offsets[s + 1]); a sequence without rows keeps its state. */
+typedef struct {
+    int32_t n_seq;          /* 1..TSV_GDN_MAX_SEQ */
+    const int32_t* offsets; /* HOST, n_seq + 1, from 0, not decreasing: the shape of the launches */
+    const int64_t* base;    /* device, n_seq: position of each sequence's first row */
+    /* device, one per row, or NULL for chains (tsv_gdn_step): the row's parent within its sequence, -1 for none; what names no
+     * earlier row of the sequence counts as -1 */
+    const int32_t* parent;
+} tsv_gdn_batch;
+
+/* The convolution's part for prompts: out gets channels values a row (unit q, unit k, v) in the rows' type, g and beta (f32,
+ * rows x n_v_heads) the decays and betas; the last conv_width - 1 rows of every sequence go to its ring. */
+typedef struct {
+    const void* qkv;
+    int64_t qkv_stride;
+    const void *a, *b;   /* n_v_heads a row */
+    int64_t gate_stride; /* of a and b; any value >= n_v_heads */
+    void* ring;
+    void* out;
+    int64_t out_stride;
+    float *g, *beta;
+} tsv_gdn_conv_io;
+int32_t tsv_gdn_conv(void* stream, const tsv_gdn_layer* layer, const tsv_gdn_batch* batch, const tsv_gdn_conv_io* io);
+
+/* The delta rule over prompts of any length, in blocks of 64 rows: state_out becomes the state behind each sequence's last row.
+ * q, k: n_k_heads x k_dim a row, of unit length or shorter (the blocks' solution is built on that); v: n_v_heads x v_dim; g (a
+ * value above 0 counts as 0) and beta as tsv_gdn_conv leaves them.  out: n_v_heads x v_dim a row; z NULL: o as it is.  The norm is
+ * taken of o as rounded to the rows' type.  The workspace (device, 16-byte aligned) belongs to the call until it has run: calls
+ * that may overlap in time take one each. */
+typedef struct {
+    const void *q, *k, *v;
+    int64_t q_stride, k_stride, v_stride;
+    const float *g, *beta;
+    const void* z;
+    int64_t z_stride;
+    const float* state_in;
+    float* state_out;
+    void* out;
+    int64_t out_stride;
+    void* workspace;
+    int64_t workspace_bytes;
+} tsv_gdn_prefill_io;
+int64_t tsv_gdn_prefill_workspace(const tsv_gdn_layer* layer, const tsv_gdn_batch* batch); /* bytes; -1: a refusal */
+int32_t tsv_gdn_prefill(void* stream, const tsv_gdn_layer* layer, const tsv_gdn_batch* batch, const tsv_gdn_prefill_io* io);
+
+/* The whole mixer for 1..TSV_MAX_ROWS rows a sequence, one launch: convolution, unit vectors, gates, the rule and the gated norm.
+ * Row i of a sequence continues the state of its parent (chain: of row i - 1; a row without one: the sequence's state).  The raw
+ * rows go to ring slots (base + i) % TSV_GDN_RING.  state_out (chains only): the state behind the last row, for rows that are
+ * final.  record: what tsv_gdn_commit needs of rows that may be rejected, with the state left as it is.  Either may be NULL.
+ * record holds f32: u (rows x n_v_heads x v_dim), the unit k (rows x n_k_heads x k_dim), g (rows x n_v_heads). */
+typedef struct {
+    const void* qkv;
+    int64_t qkv_stride;
+    const void *a, *b;
+    int64_t gate_stride;
+    const void* z; /* NULL: o as it is */
+    int64_t z_stride;
+    void* ring;
+    const float* state_in;
+    float* state_out;
+    float* record;
+    void* out;
+    int64_t out_stride;
+} tsv_gdn_step_io;
+int64_t tsv_gdn_record_bytes(const tsv_gdn_layer* layer, int64_t rows); /* -1: a refusal */
+int32_t tsv_gdn_step(void* stream, const tsv_gdn_layer* layer, const tsv_gdn_batch* batch, const tsv_gdn_step_io* io);
+
+/* commit_pending for recurrent state: of every sequence the rows the acceptance kept, path[0 .. committed] of its result (a path
+ * is cut where it stops naming rows of the sequence in ascending order; none are kept of a result with path_len 0), go into the
+ * state in path order, in n_layers layers by one launch, and their raw rows to ring slots (base + 0 ..) % TSV_GDN_RING.  batch is
+ * that of the steps (its parent is not read), results the tsv_round_result of every sequence in DEVICE memory, as
+ * tsv_accept_greedy_noalloc leaves it; record, states and rings are the first layer's, the strides lead from layer to layer
+ * (record_stride in bytes, a multiple of 4; ring_stride and state_stride in elements, multiples of 8 and 4).  Slots of ring_out
+ * that no kept row goes to are left as they are. */
+typedef struct {
+    int32_t n_layers;
+    const tsv_round_result* results;
+    const float* record;
+    int64_t record_stride;
+    const void* ring_in;
+    void* ring_out;
+    int64_t ring_stride;
+    const float* state_in;
+    float* state_out;
+    int64_t state_stride;
+} tsv_gdn_commit_io;
+int32_t tsv_gdn_commit(void* stream, const tsv_gdn_layer* layer, const tsv_gdn_batch* batch, const tsv_gdn_commit_io* io);
+
 /* ---- GGUF intake (host) -------------------------------------------------------- */
 /* The header parser of crates/repack/src/gguf_header/parser.rs:124-239 over a read-only mapping of
  * the file: version 3 only, metadata keys and tensor names unique, at most four non-zero

@@ -1,0 +1,123 @@
+"""What tsv_gdn_* refuse before any device call, and their host arithmetic: no GPU needed."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import turbospark_amd as ts
+from turbospark_amd import ffi
+
+P = 1 << 20          # stands for a device address: nothing here gets as far as reading it
+INVALID, UNSUPPORTED = -1, -3
+
+
+def _layer(**over):
+    f = dict(n_k_heads=2, n_v_heads=4, k_dim=64, v_dim=32, conv_width=4, dtype=ts.BF16, scale=0.0, l2_eps=1e-6, norm_eps=1e-6,
+             conv=P, a_log=P, dt_bias=P, norm=P)
+    f.update(over)
+    return ffi.GdnLayer(**f)
+
+
+def _batch(offsets=(0, 3), **over):
+    off = (C.c_int32 * len(offsets))(*offsets)
+    f = dict(n_seq=len(offsets) - 1, offsets=off, base=P, parent=None)
+    f.update(over)
+    b = ffi.GdnBatch(**f)
+    b.keep = off
+    return b
+
+
+CH = 2 * 2 * 64 + 4 * 32
+IO = {
+    "conv": lambda: ffi.GdnConv(qkv=P, qkv_stride=CH, a=P, b=P, gate_stride=4, ring=P, out=2 * P, out_stride=CH, g=P, beta=P),
+    "prefill": lambda: ffi.GdnPrefill(q=P, k=P, v=P, q_stride=128, k_stride=128, v_stride=128, g=P, beta=P, z=P, z_stride=128,
+                                      state_in=P, state_out=P, out=2 * P, out_stride=128, workspace=P, workspace_bytes=1 << 30),
+    "step": lambda: ffi.GdnStep(qkv=P, qkv_stride=CH, a=P, b=P, gate_stride=4, z=P, z_stride=128, ring=P, state_in=P, state_out=P,
+                                record=P, out=2 * P, out_stride=128),
+    "commit": lambda: ffi.GdnCommit(n_layers=2, results=P, record=P, record_stride=1 << 20, ring_in=P, ring_out=P, ring_stride=1 << 20,
+                                    state_in=P, state_out=P, state_stride=1 << 20),
+}
+
+
+def _call(what, layer=None, batch=None, io=None):
+    ref = lambda x: C.byref(x) if x is not None else None  # noqa: E731
+    return getattr(ffi.lib(), "tsv_gdn_" + what)(None, ref(layer), ref(batch), ref(io))
+
+
+@pytest.mark.parametrize("what", sorted(IO))
+def test_descriptions_are_refused_by_name(what):
+    refused = [
+        (INVALID, "null", dict(layer=None)), (INVALID, "null", dict(batch=None)), (INVALID, "null", dict(io=None)),
+        (INVALID, "heads", dict(layer=_layer(n_v_heads=3))), (INVALID, "heads", dict(layer=_layer(n_k_heads=0))),
+        (INVALID, "heads", dict(layer=_layer(n_k_heads=2, n_v_heads=2048))),
+        (UNSUPPORTED, "k_dim", dict(layer=_layer(k_dim=96))), (UNSUPPORTED, "v_dim", dict(layer=_layer(v_dim=24))),
+        (UNSUPPORTED, "v_dim", dict(layer=_layer(v_dim=272))), (UNSUPPORTED, "rows", dict(layer=_layer(dtype=ts.F32))),
+        (UNSUPPORTED, "taps", dict(layer=_layer(conv_width=5))), (UNSUPPORTED, "taps", dict(layer=_layer(conv_width=0))),
+        (INVALID, "epsilon", dict(layer=_layer(l2_eps=float("nan")))), (INVALID, "epsilon", dict(layer=_layer(norm_eps=-1.0))),
+        (INVALID, "batch", dict(batch=_batch(base=None))), (INVALID, "batch", dict(batch=_batch(offsets=(0, 3), base=P + 4))),
+        (INVALID, "256 sequences", dict(batch=_batch(n_seq=0))), (INVALID, "256 sequences", dict(batch=_batch(offsets=[0] * 258))),
+        (INVALID, "start at 0", dict(batch=_batch(offsets=(1, 3)))), (INVALID, "decrease", dict(batch=_batch(offsets=(0, 3, 2)))),
+    ]
+    for code, text, over in refused:
+        given = dict(layer=_layer(), batch=_batch(), io=IO[what]())
+        given.update(over)
+        assert _call(what, **given) == code, (text, over)
+        assert text in ffi.last_error() and "gdn_" + what in ffi.last_error(), ffi.last_error()
+
+
+@pytest.mark.parametrize("what,fields", [
+    ("conv", dict(qkv=None)), ("conv", dict(qkv=P + 8)), ("conv", dict(qkv_stride=CH - 8)), ("conv", dict(qkv_stride=CH + 4)),
+    ("conv", dict(out=P)), ("conv", dict(out_stride=8)), ("conv", dict(ring=None)), ("conv", dict(ring=P + 2)), ("conv", dict(gate_stride=3)),
+    ("conv", dict(a=None)), ("conv", dict(g=None)), ("conv", dict(beta=None)),
+    ("prefill", dict(q=None)), ("prefill", dict(k=P + 2)), ("prefill", dict(v_stride=120)), ("prefill", dict(out=P)),
+    ("prefill", dict(state_in=None)), ("prefill", dict(state_out=P + 64)), ("prefill", dict(workspace=None)),
+    ("prefill", dict(workspace_bytes=100)), ("prefill", dict(workspace=P + 4)), ("prefill", dict(z_stride=4)), ("prefill", dict(g=None)),
+    ("step", dict(qkv=None)), ("step", dict(out=2 * P + 2)), ("step", dict(state_in=None)), ("step", dict(state_out=P + 64)),
+    ("step", dict(z=P + 4)), ("step", dict(ring=None)), ("step", dict(b=None)), ("step", dict(record=P + 2)),
+    ("commit", dict(n_layers=0)), ("commit", dict(results=None)), ("commit", dict(results=P + 4)), ("commit", dict(record=None)),
+    ("commit", dict(ring_out=P + 64)), ("commit", dict(state_out=P + 64)), ("commit", dict(state_stride=8)), ("commit", dict(ring_stride=8)),
+    ("commit", dict(record_stride=16)), ("commit", dict(record_stride=(1 << 20) + 2)), ("commit", dict(state_in=None)),
+])
+def test_buffers_are_refused_by_name(what, fields):
+    io = IO[what]()
+    for k, v in fields.items():
+        setattr(io, k, v)
+    assert _call(what, _layer(), _batch(), io) == INVALID
+    assert "gdn_" + what in ffi.last_error()
+
+
+def test_rows_beyond_a_pass_and_trees_out_of_place_are_refused():
+    assert _call("step", _layer(), _batch(offsets=(0, 17)), IO["step"]()) == INVALID and "16 rows" in ffi.last_error()
+    assert _call("commit", _layer(), _batch(offsets=(0, 4, 21)), IO["commit"]()) == INVALID and "16 rows" in ffi.last_error()
+    assert _call("step", _layer(), _batch(parent=P), IO["step"]()) == INVALID and "tree" in ffi.last_error()
+    for what in ("conv", "prefill"):
+        assert _call(what, _layer(), _batch(parent=P), IO[what]()) == INVALID and "chains" in ffi.last_error()
+    for what in ("conv", "step"):
+        assert _call(what, _layer(conv=None), _batch(), IO[what]()) == INVALID and "null" in ffi.last_error()
+    for what in ("prefill", "step"):
+        assert _call(what, _layer(norm=None), _batch(), IO[what]()) == INVALID and "null" in ffi.last_error()
+
+
+def test_sizes_of_workspace_and_record():
+    L = ffi.lib()
+    one = L.tsv_gdn_prefill_workspace(C.byref(_layer()), C.byref(_batch(offsets=(0, 64))))
+    assert one > 0
+    assert L.tsv_gdn_prefill_workspace(C.byref(_layer()), C.byref(_batch(offsets=(0, 65)))) == 2 * one
+    assert L.tsv_gdn_prefill_workspace(C.byref(_layer()), C.byref(_batch(offsets=(0, 1, 1, 2)))) == 2 * one
+    assert L.tsv_gdn_prefill_workspace(C.byref(_layer()), C.byref(_batch(offsets=(0, 0)))) > 0
+    assert L.tsv_gdn_prefill_workspace(C.byref(_layer(k_dim=65)), C.byref(_batch())) == -1 and "k_dim" in ffi.last_error()
+    # beyond 32 bits: a long prompt of many heads
+    many = _layer(n_k_heads=64, n_v_heads=64, k_dim=256)
+    assert L.tsv_gdn_prefill_workspace(C.byref(many), C.byref(_batch(offsets=(0, 1 << 22)))) > 1 << 34
+    assert L.tsv_gdn_record_bytes(C.byref(_layer()), 5) == 4 * 5 * (4 * 32 + 2 * 64 + 4)
+    assert L.tsv_gdn_record_bytes(C.byref(_layer()), -1) == -1
+    with pytest.raises(ffi.TsvError):
+        ts.GatedDelta(2, 3, 64, 32, 4, ts.BF16).record_bytes(1)
+    with pytest.raises(ValueError):
+        ts.GatedDelta(2, 4, 64, 32, 4, ts.BF16).batch([0], P)
+
+
+def test_struct_layouts_match_the_header():
+    assert C.sizeof(ffi.GdnLayer) == 9 * 4 + 4 + 4 * 8 and C.sizeof(ffi.GdnBatch) == 4 * 8
+    assert (C.sizeof(ffi.GdnConv), C.sizeof(ffi.GdnPrefill), C.sizeof(ffi.GdnStep), C.sizeof(ffi.GdnCommit)) == (80, 128, 104, 80)
+    assert np.dtype(np.int32).itemsize * 28 == C.sizeof(ffi.RoundResultC)

@@ -1,0 +1,75 @@
+// What the kernels of a recurrent layer's mixer share: gdn.hip (convolution, few-row step, commit, the entry points) and
+// gdn_prefill.hip (the rule over prompts).
+#pragma once
+#include "tsv_internal.h"
+
+namespace tsv {
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float gf4 __attribute__((ext_vector_type(4)));
+typedef float uf4 __attribute__((ext_vector_type(4), aligned(4)));  // where only the 4-byte values are aligned
+
+// The batch as a kernel gets it: the offsets by value, so that a launch needs no copy and no host memory.
+struct GdnBatch {
+    int32_t n_seq;
+    const int64_t* base;
+    const int32_t* parent;
+    int32_t off[TSV_GDN_MAX_SEQ + 1];
+};
+
+struct GdnShape {
+    int32_t hk, hv, rep, dv, taps, channels;
+    float scale, l2_eps, norm_eps;
+    const float *conv, *a_log, *dt_bias, *norm;
+};
+
+int gdn_check(const char* who, void* stream, const tsv_gdn_layer* l, const tsv_gdn_batch* b, int max_rows, GdnShape* sh, GdnBatch* kb);
+int gdn_check_layer(const char* who, const tsv_gdn_layer* l, GdnShape* sh);
+int gdn_refuse(const char* who, const char* what);
+bool gdn_rows_ok(const void* p, int64_t stride, int64_t width);
+bool gdn_overlap(const void* a, const void* b, size_t bytes);
+
+// One row value: bf16 and fp16 bits to f32 and back (to nearest even).
+template <bool F16>
+__device__ __forceinline__ float row_f32(uint16_t b) {
+    if constexpr (F16) return (float)__builtin_bit_cast(_Float16, b);
+    return __uint_as_float((uint32_t)b << 16);
+}
+template <bool F16>
+__device__ __forceinline__ uint16_t row_bits(float x) {
+    if constexpr (F16) return __builtin_bit_cast(uint16_t, (_Float16)x);
+    return __builtin_bit_cast(uint16_t, (__bf16)x);
+}
+template <bool F16>
+__device__ __forceinline__ void row8_f32(const uint4& u, float* x) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        x[2 * i] = row_f32<F16>((uint16_t)w[i]);
+        x[2 * i + 1] = row_f32<F16>((uint16_t)(w[i] >> 16));
+    }
+}
+
+// x as two bf16 terms: x - hi - lo is at most 2^-18 of x.  Products of two such pairs without the lo * lo part are 2^-16 to 2^-17
+// off at the very most and 2^-19 on average, which is what the f32 state and the f32 record need (one term: 2^-9).
+__device__ __forceinline__ void split2(float x, __bf16& hi, __bf16& lo) {
+    hi = (__bf16)x;
+    lo = (__bf16)(x - (float)hi);
+}
+
+__device__ __forceinline__ gf4 mfma_bf16(bf16x8 a, bf16x8 b, gf4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ gf4 mfma_f32(float a, float b, gf4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ float silu_f32(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
+__device__ __forceinline__ float sigmoid_f32(float x) { return 1.0f / (1.0f + expf(-x)); }
+__device__ __forceinline__ float decay_of(float a_log, float x) {
+    return -expf(a_log) * (fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
+}
+
+// orders a wave's own LDS writes before its own later reads, where no other wave is involved
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+}  // namespace tsv

@@ -1,0 +1,728 @@
+// The mixer of a gated-delta-rule layer: the prompt's short convolution, the step of a few rows (decode and verify passes) and the
+// commit of accepted rows; entry points and argument checks of those and of the rule over prompts (gdn_prefill.hip).  Formulas:
+// include/tsverify.h.
+#include "gdn.h"
+
+#include <cstring>
+
+namespace tsv {
+
+// ---- the short convolution of prompt rows ---------------------------------------------------------------------------------
+// A thread owns 8 neighbouring channels and walks CONV_ROWS rows of them with the taps' rows in registers, so that every row is
+// read once (and conv_width - 1 of them again per tile); the k_dim / 8 threads of a head are neighbours in a wave and sum its
+// squares by lane exchange.  Bound by memory: 4 bytes a channel.
+constexpr int CONV_ROWS = 16, CONV_THREADS = 256;
+
+struct ConvArgs {
+    const uint16_t* qkv;
+    int64_t qkv_stride;
+    const uint16_t *a, *b;
+    int64_t gate_stride;
+    uint16_t* ring;
+    uint16_t* out;
+    int64_t out_stride;
+    float *g, *beta;
+    int32_t tile_of[TSV_GDN_MAX_SEQ + 1];  // first row tile of every sequence
+    int32_t channel_blocks;
+};
+
+template <int DK, bool F16>
+__global__ __launch_bounds__(CONV_THREADS) void k_gdn_conv(GdnShape sh, GdnBatch bt, ConvArgs p) {
+    int lo = 0, hi = bt.n_seq;  // the sequence of this tile: the last one that starts at or before it
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (p.tile_of[mid] <= (int)blockIdx.x) lo = mid;
+        else hi = mid;
+    }
+    const int s = lo, first = bt.off[s], n = bt.off[s + 1] - first, r0 = ((int)blockIdx.x - p.tile_of[s]) * CONV_ROWS;
+    const int rows = min(CONV_ROWS, n - r0);
+    const int64_t base = bt.base[s];
+    if ((int)blockIdx.y == p.channel_blocks) {  // the gates' block
+        for (int i = threadIdx.x; i < rows * sh.hv; i += CONV_THREADS) {
+            const int r = i / sh.hv, h = i - r * sh.hv;
+            const int64_t row = first + r0 + r;
+            p.g[row * sh.hv + h] = decay_of(sh.a_log[h], row_f32<F16>(p.a[row * p.gate_stride + h]) + sh.dt_bias[h]);
+            p.beta[row * sh.hv + h] = sigmoid_f32(row_f32<F16>(p.b[row * p.gate_stride + h]));
+        }
+        return;
+    }
+    const int c = ((int)blockIdx.y * CONV_THREADS + threadIdx.x) * 8;
+    if (c >= sh.channels) return;  // (a head's threads stay or leave together: head widths are multiples of 16 channels)
+    const int taps = sh.taps;
+    float w[4][8], x[4][8];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[j][e] = j < taps ? sh.conv[(int64_t)(c + e) * taps + taps - 1 - j] : 0.0f;  // w[j]: j rows back
+    uint16_t* ring = p.ring + (int64_t)s * TSV_GDN_RING * sh.channels + c;
+#pragma unroll
+    for (int j = 1; j < 4; j++) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (j < taps) {
+            if (r0 - j >= 0) u = *(const uint4*)(p.qkv + (int64_t)(first + r0 - j) * p.qkv_stride + c);
+            else if (base + r0 - j >= 0) u = *(const uint4*)(ring + ((base + r0 - j) & (TSV_GDN_RING - 1)) * sh.channels);
+        }
+        row8_f32<F16>(u, x[j]);
+    }
+    const bool unit = c < 2 * sh.hk * DK;
+    for (int r = 0; r < rows; r++) {
+        const int64_t row = first + r0 + r;
+        row8_f32<F16>(*(const uint4*)(p.qkv + row * p.qkv_stride + c), x[0]);
+        float y[8], sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            float v = x[0][e] * w[0][e];
+#pragma unroll
+            for (int j = 1; j < 4; j++) v = fmaf(x[j][e], w[j][e], v);
+            y[e] = silu_f32(v);
+            sum = fmaf(y[e], y[e], sum);
+        }
+        if (unit) {
+#pragma unroll
+            for (int d = 1; d < DK / 8; d <<= 1) sum += __shfl_xor(sum, d);
+            const float f = rsqrtf(sum + sh.l2_eps);
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] *= f;
+        }
+        uint4 o;
+        o.x = row_bits<F16>(y[0]) | (uint32_t)row_bits<F16>(y[1]) << 16;
+        o.y = row_bits<F16>(y[2]) | (uint32_t)row_bits<F16>(y[3]) << 16;
+        o.z = row_bits<F16>(y[4]) | (uint32_t)row_bits<F16>(y[5]) << 16;
+        o.w = row_bits<F16>(y[6]) | (uint32_t)row_bits<F16>(y[7]) << 16;
+        *(uint4*)(p.out + row * p.out_stride + c) = o;
+#pragma unroll
+        for (int j = 3; j > 0; j--)
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[j][e] = x[j - 1][e];
+    }
+    // the ring's new rows, by the thread that has read the old ones of these channels
+    if (r0 == 0)
+        for (int j = 1; j < taps && j <= n; j++)
+            *(uint4*)(ring + ((base + n - j) & (TSV_GDN_RING - 1)) * sh.channels) = *(const uint4*)(p.qkv + (int64_t)(first + n - j) * p.qkv_stride + c);
+}
+
+// ---- the step of a few rows -------------------------------------------------------------------------------------------------
+// One workgroup per (value head, sequence), a wave per 16 value channels.  A wave's part of the state (16 x k_dim f32) is asked
+// for first and stays in registers; what the rows need beside it is made meanwhile: the convolution of the head's q, k and v
+// channels, the unit vectors as two bf16 terms in operand order, D_ij = exp(sum of g from j, exclusive, to i) along the root
+// paths, and from D and the products k_i.k_j, q_i.k_j the 16 x 16 matrices
+//     T = (I + A)^-1,  A_ij = beta_i D_ij k_i.k_j (j a strict ancestor of i),    P_ij = D_ij q_i.k_j (j an ancestor or i).
+// Then, for all rows at once: KS = k S, QS = q S (three bf16 products each: 2^-17, see split2), u = T beta (v - e^G KS),
+// o = e^G QS + P u, and for final rows S <- e^G_end S + sum_i D_end,i k_i u_i (f32 matrix instructions).  With many sequences the
+// state's bytes bound it, with one the chain of loads and barriers.
+// Operand order of the contraction over k_dim: lane group gq of the 16x16x32 instruction takes elements 4 gq .. + 3 of both
+// 16-wide halves of its 32, so that two neighbouring D tiles of the f32 update are exactly one B operand.
+
+struct StepArgs {
+    const uint16_t* qkv;
+    int64_t qkv_stride;
+    const uint16_t *a, *b;
+    int64_t gate_stride;
+    const uint16_t* z;
+    int64_t z_stride;
+    uint16_t* ring;
+    const float* state_in;
+    float* state_out;
+    float* record;
+    uint16_t* out;
+    int64_t out_stride;
+    int32_t total_rows, max_rows;
+};
+
+template <int DK, bool F16, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_gdn_step(GdnShape sh, GdnBatch bt, StepArgs p) {
+    extern __shared__ uint4 step_lds[];
+    const int h = blockIdx.x, s = blockIdx.y, hk = h / sh.rep, dv = sh.dv, nt = blockDim.x, tid = threadIdx.x;
+    const int lane = tid & 63, wave = tid >> 6, l16 = lane & 15, gq = lane >> 4;
+    const int first = bt.off[s], m = bt.off[s + 1] - first, taps = sh.taps;
+    const int64_t base = bt.base[s];
+    const size_t at = ((size_t)s * sh.hv + h) * dv * DK + (size_t)(16 * wave + l16) * DK + 4 * gq;
+    constexpr int NT = DK / 16;
+    float4 S[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) S[t] = *(const float4*)(p.state_in + at + 16 * t);
+    if (m <= 0) {  // no rows: the state stays
+        if (p.state_out) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) *(float4*)(p.state_out + at + 16 * t) = base == 0 ? make_float4(0, 0, 0, 0) : S[t];
+        }
+        return;
+    }
+    // LDS: the convolved rows, the operand fragments (or, before them, the raw rows), the small matrices
+    const int cn = 2 * DK + dv, mr = p.max_rows;
+    float* ys = (float*)step_lds;                          // [row][q | k | v]
+    float* xs = ys + mr * cn;                              // [taps - 1 + row][..], dead once convolved
+    uint4* kf = (uint4*)xs;                                // [q, k][hi, lo][DK / 32][lane]
+    constexpr int FR = DK / 32 * 64;
+    const int big = max((taps - 1 + mr) * cn, 16 * FR);
+    float* D = xs + big;                                   // [16][16], zero where j is no ancestor of i
+    float* A = D + 256;                                    // [16][20]
+    float* T = A + 320;
+    float* P = T + 320;
+    float* beta = P + 320;
+    float* eG = beta + 16;
+    float* gs = eG + 16;
+    float* red = gs + 16;                                  // [wave][16]
+    int* par = (int*)(red + 16 * (nt >> 6));
+    int* anc = par + 16;                                   // [16][4]: the row j steps back, as a row of xs
+    if (tid < 16) {
+        const int i = tid;
+        float g = 0.0f, be = 0.0f;
+        int pr = i - 1;
+        if (i < m) {
+            const int64_t row = first + i;
+            g = decay_of(sh.a_log[h], row_f32<F16>(p.a[row * p.gate_stride + h]) + sh.dt_bias[h]);
+            be = sigmoid_f32(row_f32<F16>(p.b[row * p.gate_stride + h]));
+            if (bt.parent) {
+                pr = bt.parent[row];
+                if (pr < 0 || pr >= i) pr = -1;
+            }
+            if (p.record) p.record[(size_t)p.total_rows * (sh.hv * dv + sh.hk * DK) + (size_t)row * sh.hv + h] = g;
+        }
+        gs[i] = g;
+        beta[i] = be;
+        par[i] = pr;
+    }
+    // the raw rows of this head's channels, history first; they go to their ring slots on the way
+    const int pieces = cn >> 3;
+    uint16_t* ring = p.ring + (int64_t)s * TSV_GDN_RING * sh.channels;
+    for (int i = tid; i < (taps - 1 + m) * pieces; i += nt) {
+        const int r = i / pieces, c = (i - r * pieces) * 8;
+        const int ch = c < DK ? hk * DK + c : c < 2 * DK ? (sh.hk + hk) * DK + c - DK : 2 * sh.hk * DK + h * dv + c - 2 * DK;
+        const int back = r - (taps - 1);
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (back >= 0) {
+            u = *(const uint4*)(p.qkv + (int64_t)(first + back) * p.qkv_stride + ch);
+            if (c >= 2 * DK || h == hk * sh.rep) *(uint4*)(ring + ((base + back) & (TSV_GDN_RING - 1)) * sh.channels + ch) = u;
+        } else if (base + back >= 0) {
+            u = *(const uint4*)(ring + ((base + back) & (TSV_GDN_RING - 1)) * sh.channels + ch);
+        }
+        row8_f32<F16>(u, xs + r * cn + c);
+    }
+    __syncthreads();
+    if (tid < 16) {
+        const int i = tid;
+        int q = i;
+        float sum = 0.0f;
+        for (int j = 0; j < 16; j++) D[i * 16 + j] = 0.0f;
+        for (int at_row = i; at_row >= 0; at_row = par[at_row]) {  // parents come before their children: at most 16 steps
+            D[i * 16 + at_row] = expf(sum);
+            sum += gs[at_row];
+        }
+        eG[i] = expf(sum);
+        for (int j = 0; j < 4; j++) {
+            anc[i * 4 + j] = max(q + taps - 1, 0);
+            q = q >= 0 ? par[q] : q - 1;
+        }
+    }
+    __syncthreads();
+    for (int c = tid; c < cn; c += nt) {
+        const int ch = c < DK ? hk * DK + c : c < 2 * DK ? (sh.hk + hk) * DK + c - DK : 2 * sh.hk * DK + h * dv + c - 2 * DK;
+        float w[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = j < taps ? sh.conv[(int64_t)ch * taps + taps - 1 - j] : 0.0f;
+        for (int i = 0; i < m; i++) {
+            float v = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (j < taps) v = fmaf(xs[anc[i * 4 + j] * cn + c], w[j], v);
+            ys[i * cn + c] = silu_f32(v);
+        }
+    }
+    __syncthreads();
+    // unit vectors, as f32 (k, for the update and the record) and as operand fragments
+    for (int i = tid; i < 4 * DK; i += nt) {
+        const int mat = i / (2 * DK), row = (i / (DK / 8)) & 15, c8 = i & (DK / 8 - 1);
+        float x[8], sum = 0.0f;
+        float* src = ys + row * cn + mat * DK + 8 * c8;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = row < m ? src[e] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum = fmaf(x[e], x[e], sum);
+#pragma unroll
+        for (int d = 1; d < DK / 8; d <<= 1) sum += __shfl_xor(sum, d);
+        const float f = row < m ? rsqrtf(sum + sh.l2_eps) : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] *= f;
+        if (mat == 1 && row < m) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) src[e] = x[e];
+            if (p.record && h == hk * sh.rep) {
+                float* to = p.record + (size_t)p.total_rows * sh.hv * dv + ((size_t)(first + row) * sh.hk + hk) * DK + 8 * c8;
+#pragma unroll
+                for (int e = 0; e < 8; e++) to[e] = x[e];
+            }
+        }
+        const int step = c8 >> 2;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int o = 8 * (c8 & 3) + 4 * e, to = (step * 64 + ((o & 15) >> 2) * 16 + row) * 2 + (o >> 4);
+            __bf16 hi[4], lo[4];
+#pragma unroll
+            for (int y = 0; y < 4; y++) split2(x[4 * e + y], hi[y], lo[y]);
+            uint2* f2 = (uint2*)(kf + mat * 2 * FR);
+            f2[to] = *(uint2*)hi;
+            f2[2 * FR + to] = *(uint2*)lo;
+        }
+    }
+    __syncthreads();
+    const uint4 *qh = kf, *ql = kf + FR, *kh = kf + 2 * FR, *kl = kf + 3 * FR;
+    const int waves = nt >> 6;
+    if (wave == 0 || wave == 1 || waves == 1) {
+        for (int which = wave; which < 2; which += waves) {  // 0: k.k -> A, T;  1: q.k -> P
+            gf4 acc = {0, 0, 0, 0};
+#pragma unroll
+            for (int t = 0; t < DK / 32; t++) {
+                const bf16x8 bh = __builtin_bit_cast(bf16x8, kh[t * 64 + lane]), bl = __builtin_bit_cast(bf16x8, kl[t * 64 + lane]);
+                const bf16x8 ah = __builtin_bit_cast(bf16x8, (which ? qh : kh)[t * 64 + lane]);
+                const bf16x8 al = __builtin_bit_cast(bf16x8, (which ? ql : kl)[t * 64 + lane]);
+                acc = mfma_bf16(ah, bh, acc);
+                acc = mfma_bf16(ah, bl, acc);
+                acc = mfma_bf16(al, bh, acc);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const int i = 4 * gq + r;
+                const float d = D[i * 16 + l16] * acc[r];
+                if (which) P[i * 20 + l16] = d;
+                else A[i * 20 + l16] = i == l16 ? 0.0f : beta[i] * d;
+            }
+            if (which == 0) {
+                wave_lds_fence();
+                float x[16];  // column l16 of T, row after row
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float v = i == l16 ? 1.0f : 0.0f;
+                    if (i < m) {
+#pragma unroll
+                        for (int j = 0; j < i; j++) v = fmaf(-A[i * 20 + j], x[j], v);
+                    }
+                    x[i] = v;
+                    if (gq == 0) T[i * 20 + l16] = v;
+                }
+            }
+        }
+    }
+    __syncthreads();
+    if (base == 0) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) S[t] = make_float4(0, 0, 0, 0);
+    }
+    gf4 ks = {0, 0, 0, 0}, qs = {0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < DK / 32; t++) {
+        bf16x8 sh8, sl8;
+        const float sv[8] = {S[2 * t].x, S[2 * t].y, S[2 * t].z, S[2 * t].w, S[2 * t + 1].x, S[2 * t + 1].y, S[2 * t + 1].z, S[2 * t + 1].w};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            __bf16 hi, lo;
+            split2(sv[e], hi, lo);
+            sh8[e] = hi;
+            sl8[e] = lo;
+        }
+        const bf16x8 k0 = __builtin_bit_cast(bf16x8, kh[t * 64 + lane]), k1 = __builtin_bit_cast(bf16x8, kl[t * 64 + lane]);
+        const bf16x8 q0 = __builtin_bit_cast(bf16x8, qh[t * 64 + lane]), q1 = __builtin_bit_cast(bf16x8, ql[t * 64 + lane]);
+        ks = mfma_bf16(k0, sh8, ks);
+        qs = mfma_bf16(q0, sh8, qs);
+        ks = mfma_bf16(k0, sl8, ks);
+        qs = mfma_bf16(q0, sl8, qs);
+        ks = mfma_bf16(k1, sh8, ks);
+        qs = mfma_bf16(q1, sh8, qs);
+    }
+    const int col = 16 * wave + l16;  // this lane's value channel; its rows are 4 gq .. + 3
+    gf4 u = {0, 0, 0, 0}, o = {0, 0, 0, 0};
+    const float4 t4 = *(const float4*)(T + l16 * 20 + 4 * gq), p4 = *(const float4*)(P + l16 * 20 + 4 * gq);
+    const float tt[4] = {t4.x, t4.y, t4.z, t4.w}, pp[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int i = 4 * gq + r;
+        const float v = i < m ? ys[i * cn + 2 * DK + col] : 0.0f;
+        u = mfma_f32(tt[r], beta[i] * fmaf(-eG[i], ks[r], v), u);
+        o[r] = eG[i] * qs[r];
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) o = mfma_f32(pp[r], u[r], o);
+    if (p.record) {
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            if (4 * gq + r < m) p.record[((size_t)(first + 4 * gq + r) * sh.hv + h) * dv + col] = u[r];
+    }
+    if (p.state_out) {
+        const float end = eG[m - 1];
+        float uw[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) uw[r] = u[r] * D[(m - 1) * 16 + 4 * gq + r];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            gf4 acc = {S[t].x * end, S[t].y * end, S[t].z * end, S[t].w * end};
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (r < m) {  // (rows 4, 8 and 12 ride in the same instruction as row 0)
+                    const int i = 4 * gq + r;
+                    acc = mfma_f32(i < m ? ys[i * cn + DK + 16 * t + l16] : 0.0f, uw[r], acc);
+                }
+            *(float4*)(p.state_out + at + 16 * t) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++) o[r] *= sh.scale;
+    if (p.z) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            float q = o[r] * o[r];
+            for (int d = 1; d < 16; d <<= 1) q += __shfl_xor(q, d);
+            if (l16 == 0) red[wave * 16 + 4 * gq + r] = q;
+        }
+        __syncthreads();
+        const float nw = sh.norm[col];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int i = 4 * gq + r;
+            float sum = 0.0f;
+            for (int w = 0; w < waves; w++) sum += red[w * 16 + i];
+            if (i < m) {
+                const float z = row_f32<F16>(p.z[(int64_t)(first + i) * p.z_stride + h * dv + col]);
+                o[r] *= rsqrtf(sum / (float)dv + sh.norm_eps) * nw * silu_f32(z);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+        if (4 * gq + r < m) p.out[(int64_t)(first + 4 * gq + r) * p.out_stride + h * dv + col] = row_bits<F16>(o[r]);
+}
+
+// ---- accepted rows into the state -----------------------------------------------------------------------------------------------
+// S <- e^{g_1 + .. + g_n} S + sum_i e^{g_{i+1} + .. + g_n} k_i u_i^T over the kept path.  A thread keeps four state values of COMMIT
+// value channels and the matching k of every kept row; one pass over the state, which is what bounds it.  The last workgroups of a
+// (sequence, layer) move the ring's rows: slot i takes the row of slot path[i] >= i, in ascending order by one thread.
+constexpr int COMMIT_THREADS = 256, COMMIT_PIECES = 4;
+
+struct CommitArgs {
+    const tsv_round_result* results;
+    const float* record;
+    int64_t record_stride;  // floats
+    const uint16_t* ring_in;
+    uint16_t* ring_out;
+    int64_t ring_stride;
+    const float* state_in;
+    float* state_out;
+    int64_t state_stride;
+    int32_t total_rows, state_blocks;
+};
+
+template <int DK>
+__global__ __launch_bounds__(COMMIT_THREADS) void k_gdn_commit(GdnShape sh, GdnBatch bt, CommitArgs p) {
+    const int s = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, first = bt.off[s], m = bt.off[s + 1] - first;
+    __shared__ int said[TSV_MAX_ROWS + 2], path[TSV_MAX_ROWS], kept;
+    __shared__ float g[TSV_MAX_ROWS], w[TSV_MAX_ROWS + 1];
+    const int64_t base = bt.base[s];
+    constexpr int PER_ROW = DK / 4, CH = COMMIT_THREADS / PER_ROW * COMMIT_PIECES;  // value channels of a workgroup
+    const bool of_ring = (int)blockIdx.x >= p.state_blocks;
+    const int blocks = (sh.dv + CH - 1) / CH, h = of_ring ? 0 : (int)blockIdx.x / blocks, c0 = ((int)blockIdx.x - h * blocks) * CH;
+    const float* rec = p.record + (int64_t)layer * p.record_stride;
+    const int kq = (tid % PER_ROW) * 4;
+    const size_t at = (size_t)((int64_t)layer * p.state_stride) + ((size_t)s * sh.hv + h) * sh.dv * DK + kq;
+    float4 S[COMMIT_PIECES];
+    int ch[COMMIT_PIECES];
+#pragma unroll
+    for (int i = 0; i < COMMIT_PIECES; i++) {
+        ch[i] = of_ring ? sh.dv : c0 + tid / PER_ROW + i * (COMMIT_THREADS / PER_ROW);
+        S[i] = make_float4(0, 0, 0, 0);
+        if (ch[i] < sh.dv) S[i] = *(const float4*)(p.state_in + at + (size_t)ch[i] * DK);
+    }
+    if (tid < TSV_MAX_ROWS) {
+        said[tid] = p.results[s].path[tid];
+        g[tid] = tid < m ? rec[(size_t)p.total_rows * (sh.hv * sh.dv + sh.hk * DK) + (size_t)(first + tid) * sh.hv + h] : 0.0f;
+    } else if (tid == TSV_MAX_ROWS) {
+        said[tid] = p.results[s].path_len;
+    } else if (tid == TSV_MAX_ROWS + 1) {
+        said[tid] = p.results[s].committed;
+    }
+    __syncthreads();
+    if (tid == 0) {
+        const int rows = min(m, TSV_MAX_ROWS), len = said[TSV_MAX_ROWS];
+        const int want = min(len, said[TSV_MAX_ROWS + 1] < rows ? said[TSV_MAX_ROWS + 1] + 1 : rows);
+        int n = 0, before = -1;
+        while (n < want && said[n] > before && said[n] < rows) path[n] = before = said[n], n++;
+        kept = n;
+        float sum = 0.0f;
+        for (int i = n - 1; i >= 0; i--) {
+            w[i] = expf(sum);
+            sum += g[path[i]];
+        }
+        w[TSV_MAX_ROWS] = expf(sum);
+    }
+    __syncthreads();
+    const int n = kept;
+    if (of_ring) {
+        const int c = (((int)blockIdx.x - p.state_blocks) * COMMIT_THREADS + tid) * 8;
+        if (c >= sh.channels) return;
+        const int64_t to = (int64_t)layer * p.ring_stride + (int64_t)s * TSV_GDN_RING * sh.channels + c;
+        for (int i = 0; i < n; i++) {
+            if (path[i] == i && p.ring_in == p.ring_out) continue;
+            *(uint4*)(p.ring_out + to + ((base + i) & (TSV_GDN_RING - 1)) * sh.channels) =
+                *(const uint4*)(p.ring_in + to + ((base + path[i]) & (TSV_GDN_RING - 1)) * sh.channels);
+        }
+        return;
+    }
+    const float end = w[TSV_MAX_ROWS];
+#pragma unroll
+    for (int i = 0; i < COMMIT_PIECES; i++) {
+        if (base == 0) S[i] = make_float4(0, 0, 0, 0);  // (what the buffer holds may be no number)
+        S[i].x *= end;
+        S[i].y *= end;
+        S[i].z *= end;
+        S[i].w *= end;
+    }
+    for (int j = 0; j < n; j++) {
+        const size_t row = first + path[j];
+        const uf4 k = *(const uf4*)(rec + (size_t)p.total_rows * sh.hv * sh.dv + (row * sh.hk + h / sh.rep) * DK + kq);
+        const float wj = w[j];
+#pragma unroll
+        for (int i = 0; i < COMMIT_PIECES; i++) {
+            const float u = ch[i] < sh.dv ? wj * rec[(row * sh.hv + h) * sh.dv + ch[i]] : 0.0f;
+            S[i].x = fmaf(u, k.x, S[i].x);
+            S[i].y = fmaf(u, k.y, S[i].y);
+            S[i].z = fmaf(u, k.z, S[i].z);
+            S[i].w = fmaf(u, k.w, S[i].w);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < COMMIT_PIECES; i++)
+        if (ch[i] < sh.dv) *(float4*)(p.state_out + at + (size_t)ch[i] * DK) = S[i];
+}
+
+// ---- arguments ----------------------------------------------------------------------------------------------------------------
+
+int gdn_refuse(const char* who, const char* what) {
+    set_error(std::string(who) + ": " + what);
+    return TSV_ERR_INVALID;
+}
+
+bool gdn_rows_ok(const void* p, int64_t stride, int64_t width) {
+    return p && ((uintptr_t)p & 15) == 0 && (stride & 7) == 0 && stride >= width && stride <= (int64_t)1 << 40;
+}
+
+bool gdn_overlap(const void* a, const void* b, size_t bytes) {
+    return a != b && (uintptr_t)a < (uintptr_t)b + bytes && (uintptr_t)b < (uintptr_t)a + bytes;
+}
+
+int gdn_check_layer(const char* who, const tsv_gdn_layer* l, GdnShape* sh) {
+    if (!l) return gdn_refuse(who, "null layer");
+    if (l->n_k_heads < 1 || l->n_v_heads < 1 || l->n_v_heads % l->n_k_heads || l->n_v_heads > 1024)
+        return gdn_refuse(who, "1..1024 value heads, a multiple of the key heads");
+    if ((l->k_dim != 64 && l->k_dim != 128 && l->k_dim != 256) || l->v_dim < 16 || l->v_dim > 256 || l->v_dim % 16) {
+        set_error(std::string(who) + ": k_dim must be 64, 128 or 256, v_dim a multiple of 16 up to 256");
+        return TSV_ERR_UNSUPPORTED;
+    }
+    if (l->dtype != TSV_BF16 && l->dtype != TSV_F16) {
+        set_error(std::string(who) + ": rows are bf16 or fp16");
+        return TSV_ERR_UNSUPPORTED;
+    }
+    if (l->conv_width < 1 || l->conv_width > 4) {
+        set_error(std::string(who) + ": 1..4 convolution taps");
+        return TSV_ERR_UNSUPPORTED;
+    }
+    if (!(l->l2_eps >= 0.0f) || !(l->norm_eps >= 0.0f) || !(l->scale == l->scale)) return gdn_refuse(who, "a negative or undefined epsilon or scale");
+    sh->hk = l->n_k_heads;
+    sh->hv = l->n_v_heads;
+    sh->rep = l->n_v_heads / l->n_k_heads;
+    sh->dv = l->v_dim;
+    sh->taps = l->conv_width;
+    sh->channels = 2 * l->n_k_heads * l->k_dim + l->n_v_heads * l->v_dim;
+    sh->scale = l->scale > 0.0f ? l->scale : 1.0f / sqrtf((float)l->k_dim);
+    sh->l2_eps = l->l2_eps;
+    sh->norm_eps = l->norm_eps;
+    sh->conv = l->conv;
+    sh->a_log = l->a_log;
+    sh->dt_bias = l->dt_bias;
+    sh->norm = l->norm;
+    return TSV_OK;
+}
+
+int gdn_check(const char* who, void* stream, const tsv_gdn_layer* l, const tsv_gdn_batch* b, int max_rows, GdnShape* sh, GdnBatch* kb) {
+    const int rc = gdn_check_layer(who, l, sh);
+    if (rc) return rc;
+    if (!b || !b->offsets || !b->base || ((uintptr_t)b->base & 7) || ((uintptr_t)b->parent & 3)) return gdn_refuse(who, "null or misaligned batch");
+    if (b->n_seq < 1 || b->n_seq > TSV_GDN_MAX_SEQ) return gdn_refuse(who, "1..256 sequences");
+    if (b->offsets[0] != 0) return gdn_refuse(who, "offsets start at 0");
+    for (int s = 0; s < b->n_seq; s++) {
+        if (b->offsets[s + 1] < b->offsets[s]) return gdn_refuse(who, "offsets decrease");
+        if (max_rows && b->offsets[s + 1] - b->offsets[s] > max_rows) return gdn_refuse(who, "at most 16 rows a sequence");
+    }
+    if (b->offsets[b->n_seq] > 1 << 28) return gdn_refuse(who, "more than 2^28 rows");
+    kb->n_seq = b->n_seq;
+    kb->base = b->base;
+    kb->parent = b->parent;
+    std::memcpy(kb->off, b->offsets, sizeof(int32_t) * (b->n_seq + 1));
+    if (stream) {  // launches go to the current device
+        int current = 0;
+        hipDevice_t of = 0;
+        TSV_HIP(hipGetDevice(&current));
+        TSV_HIP(hipStreamGetDevice((hipStream_t)stream, &of));
+        if ((int)of != current) return gdn_refuse(who, "the stream belongs to another device than the current one");
+    }
+    return TSV_OK;
+}
+
+namespace {
+
+template <int DK, bool F16>
+int launch_conv(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const ConvArgs& p, int tiles) {
+    hipLaunchKernelGGL((k_gdn_conv<DK, F16>), dim3(tiles, p.channel_blocks + 1), dim3(CONV_THREADS), 0, st, sh, bt, p);
+    TSV_HIP(hipGetLastError());
+    return TSV_OK;
+}
+
+template <int DK, bool F16, int THREADS>
+int launch_step(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const StepArgs& p) {
+    const int waves = sh.dv / 16, cn = 2 * DK + sh.dv;
+    const int raw = (sh.taps - 1 + p.max_rows) * cn, frags = 16 * (DK / 32 * 64);
+    const size_t lds = sizeof(float) * (size_t)(p.max_rows * cn + (raw > frags ? raw : frags) + 256 + 3 * 320 + 3 * 16 + 16 * waves + 16 + 64);
+    static OncePerDevice once;
+    const int rc = allow_lds((const void*)k_gdn_step<DK, F16, THREADS>, lds, once);
+    if (rc) return rc;
+    hipLaunchKernelGGL((k_gdn_step<DK, F16, THREADS>), dim3(sh.hv, bt.n_seq), dim3(64 * waves), lds, st, sh, bt, p);
+    TSV_HIP(hipGetLastError());
+    return TSV_OK;
+}
+
+template <int DK>
+int launch_commit(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, CommitArgs& p, int layers) {
+    constexpr int CH = COMMIT_THREADS / (DK / 4) * COMMIT_PIECES;
+    p.state_blocks = sh.hv * ((sh.dv + CH - 1) / CH);
+    const int ring_blocks = (sh.channels / 8 + COMMIT_THREADS - 1) / COMMIT_THREADS;
+    hipLaunchKernelGGL((k_gdn_commit<DK>), dim3(p.state_blocks + ring_blocks, bt.n_seq, layers), dim3(COMMIT_THREADS), 0, st, sh, bt, p);
+    TSV_HIP(hipGetLastError());
+    return TSV_OK;
+}
+
+}  // namespace
+
+}  // namespace tsv
+
+using namespace tsv;
+
+extern "C" int32_t tsv_gdn_conv(void* stream, const tsv_gdn_layer* layer, const tsv_gdn_batch* batch, const tsv_gdn_conv_io* io) {
+    const char* who = "gdn_conv";
+    GdnShape sh;
+    GdnBatch bt;
+    const int rc = gdn_check(who, stream, layer, batch, 0, &sh, &bt);
+    if (rc) return rc;
+    if (!io || !io->a || !io->b || !io->ring || !io->g || !io->beta || !sh.conv || !sh.a_log || !sh.dt_bias) return gdn_refuse(who, "null argument");
+    if (batch->parent) return gdn_refuse(who, "prompt rows are chains");
+    if (!gdn_rows_ok(io->qkv, io->qkv_stride, sh.channels) || !gdn_rows_ok(io->out, io->out_stride, sh.channels) || ((uintptr_t)io->ring & 15) ||
+        io->gate_stride < sh.hv || ((uintptr_t)io->g & 3) || ((uintptr_t)io->beta & 3))
+        return gdn_refuse(who, "rows, rings and strides: 16-byte aligned, multiples of 8, as wide as a row");
+    if (io->out == io->qkv) return gdn_refuse(who, "out may not be the input rows");
+    ConvArgs p;
+    p.qkv = (const uint16_t*)io->qkv;
+    p.qkv_stride = io->qkv_stride;
+    p.a = (const uint16_t*)io->a;
+    p.b = (const uint16_t*)io->b;
+    p.gate_stride = io->gate_stride;
+    p.ring = (uint16_t*)io->ring;
+    p.out = (uint16_t*)io->out;
+    p.out_stride = io->out_stride;
+    p.g = io->g;
+    p.beta = io->beta;
+    p.tile_of[0] = 0;
+    for (int s = 0; s < bt.n_seq; s++) p.tile_of[s + 1] = p.tile_of[s] + (bt.off[s + 1] - bt.off[s] + CONV_ROWS - 1) / CONV_ROWS;
+    p.channel_blocks = (sh.channels / 8 + CONV_THREADS - 1) / CONV_THREADS;
+    const int tiles = p.tile_of[bt.n_seq];
+    if (!tiles) return TSV_OK;
+    const hipStream_t st = (hipStream_t)stream;
+    const bool f16 = layer->dtype == TSV_F16;
+    if (layer->k_dim == 64) return f16 ? launch_conv<64, true>(st, sh, bt, p, tiles) : launch_conv<64, false>(st, sh, bt, p, tiles);
+    if (layer->k_dim == 128) return f16 ? launch_conv<128, true>(st, sh, bt, p, tiles) : launch_conv<128, false>(st, sh, bt, p, tiles);
+    return f16 ? launch_conv<256, true>(st, sh, bt, p, tiles) : launch_conv<256, false>(st, sh, bt, p, tiles);
+}
+
+extern "C" int64_t tsv_gdn_record_bytes(const tsv_gdn_layer* layer, int64_t rows) {
+    GdnShape sh;
+    if (gdn_check_layer("gdn_record_bytes", layer, &sh)) return -1;
+    if (rows < 0 || rows > 1 << 28) {
+        gdn_refuse("gdn_record_bytes", "0..2^28 rows");
+        return -1;
+    }
+    return 4 * rows * (int64_t)(sh.hv * sh.dv + sh.hk * layer->k_dim + sh.hv);
+}
+
+extern "C" int32_t tsv_gdn_step(void* stream, const tsv_gdn_layer* layer, const tsv_gdn_batch* batch, const tsv_gdn_step_io* io) {
+    const char* who = "gdn_step";
+    GdnShape sh;
+    GdnBatch bt;
+    const int rc = gdn_check(who, stream, layer, batch, TSV_MAX_ROWS, &sh, &bt);
+    if (rc) return rc;
+    if (!io || !io->a || !io->b || !io->ring || !io->state_in || !sh.conv || !sh.a_log || !sh.dt_bias || (io->z && !sh.norm)) return gdn_refuse(who, "null argument");
+    if (!gdn_rows_ok(io->qkv, io->qkv_stride, sh.channels) || !gdn_rows_ok(io->out, io->out_stride, (int64_t)sh.hv * sh.dv) ||
+        (io->z && !gdn_rows_ok(io->z, io->z_stride, (int64_t)sh.hv * sh.dv)) || ((uintptr_t)io->ring & 15) || io->gate_stride < sh.hv ||
+        ((uintptr_t)io->state_in & 15) || ((uintptr_t)io->state_out & 15) || ((uintptr_t)io->record & 3))
+        return gdn_refuse(who, "rows, rings, states, record and strides: 16-byte aligned, multiples of 8, as wide as a row");
+    if (io->state_out && batch->parent) return gdn_refuse(who, "rows of a tree are not final: no state_out");
+    if (io->state_out && gdn_overlap(io->state_in, io->state_out, sizeof(float) * (size_t)bt.n_seq * sh.hv * sh.dv * layer->k_dim))
+        return gdn_refuse(who, "state_out overlaps state_in");
+    StepArgs p;
+    p.qkv = (const uint16_t*)io->qkv;
+    p.qkv_stride = io->qkv_stride;
+    p.a = (const uint16_t*)io->a;
+    p.b = (const uint16_t*)io->b;
+    p.gate_stride = io->gate_stride;
+    p.z = (const uint16_t*)io->z;
+    p.z_stride = io->z_stride;
+    p.ring = (uint16_t*)io->ring;
+    p.state_in = io->state_in;
+    p.state_out = io->state_out;
+    p.record = io->record;
+    p.out = (uint16_t*)io->out;
+    p.out_stride = io->out_stride;
+    p.total_rows = bt.off[bt.n_seq];
+    p.max_rows = 1;
+    for (int s = 0; s < bt.n_seq; s++) p.max_rows = std::max(p.max_rows, bt.off[s + 1] - bt.off[s]);
+    const hipStream_t st = (hipStream_t)stream;
+    const bool f16 = layer->dtype == TSV_F16, wide = sh.dv > 128;
+#define TSV_GDN_STEP(DK)                                                                                                   \
+    (wide ? (f16 ? launch_step<DK, true, 1024>(st, sh, bt, p) : launch_step<DK, false, 1024>(st, sh, bt, p))              \
+          : (f16 ? launch_step<DK, true, 512>(st, sh, bt, p) : launch_step<DK, false, 512>(st, sh, bt, p)))
+    if (layer->k_dim == 64) return TSV_GDN_STEP(64);
+    if (layer->k_dim == 128) return TSV_GDN_STEP(128);
+    return TSV_GDN_STEP(256);
+#undef TSV_GDN_STEP
+}
+
+extern "C" int32_t tsv_gdn_commit(void* stream, const tsv_gdn_layer* layer, const tsv_gdn_batch* batch, const tsv_gdn_commit_io* io) {
+    const char* who = "gdn_commit";
+    GdnShape sh;
+    GdnBatch bt;
+    const int rc = gdn_check(who, stream, layer, batch, TSV_MAX_ROWS, &sh, &bt);
+    if (rc) return rc;
+    if (!io || !io->results || !io->record || !io->ring_in || !io->ring_out || !io->state_in || !io->state_out) return gdn_refuse(who, "null argument");
+    if (io->n_layers < 1 || io->n_layers > 65535) return gdn_refuse(who, "1..65535 layers");
+    const int64_t state = (int64_t)bt.n_seq * sh.hv * sh.dv * layer->k_dim, ring = (int64_t)bt.n_seq * TSV_GDN_RING * sh.channels;
+    const int64_t rec = tsv_gdn_record_bytes(layer, bt.off[bt.n_seq]);
+    if (((uintptr_t)io->results & 7) || ((uintptr_t)io->record & 3) || ((uintptr_t)io->ring_in & 15) || ((uintptr_t)io->ring_out & 15) ||
+        ((uintptr_t)io->state_in & 15) || ((uintptr_t)io->state_out & 15))
+        return gdn_refuse(who, "misaligned argument");
+    if (io->n_layers > 1 && (io->record_stride < rec || io->record_stride & 3 || io->ring_stride < ring || io->ring_stride & 7 ||
+                             io->state_stride < state || io->state_stride & 3))
+        return gdn_refuse(who, "a layer's stride is shorter than a layer or misaligned");
+    const int64_t more = io->n_layers - 1;
+    if (gdn_overlap(io->state_in, io->state_out, sizeof(float) * (size_t)(more * io->state_stride + state)) ||
+        gdn_overlap(io->ring_in, io->ring_out, 2 * (size_t)(more * io->ring_stride + ring)))
+        return gdn_refuse(who, "state_out overlaps state_in, or ring_out ring_in");
+    CommitArgs p;
+    p.results = io->results;
+    p.record = io->record;
+    p.record_stride = more ? io->record_stride / 4 : 0;
+    p.ring_in = (const uint16_t*)io->ring_in;
+    p.ring_out = (uint16_t*)io->ring_out;
+    p.ring_stride = more ? io->ring_stride : 0;
+    p.state_in = io->state_in;
+    p.state_out = io->state_out;
+    p.state_stride = more ? io->state_stride : 0;
+    p.total_rows = bt.off[bt.n_seq];
+    const hipStream_t st = (hipStream_t)stream;
+    if (layer->k_dim == 64) return launch_commit<64>(st, sh, bt, p, io->n_layers);
+    if (layer->k_dim == 128) return launch_commit<128>(st, sh, bt, p, io->n_layers);
+    return launch_commit<256>(st, sh, bt, p, io->n_layers);
+}

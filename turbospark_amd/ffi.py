@@ -222,6 +222,44 @@ class GenerationResult(C.Structure):
                 ("reused", C.c_int64)]
 
 
+class GdnLayer(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("n_k_heads", "n_v_heads", "k_dim", "v_dim", "conv_width", "dtype")] + \
+               [(n, C.c_float) for n in ("scale", "l2_eps", "norm_eps")] + \
+               [(n, C.c_void_p) for n in ("conv", "a_log", "dt_bias", "norm")]
+
+
+class GdnBatch(C.Structure):
+    _fields_ = [("n_seq", C.c_int32), ("offsets", C.POINTER(C.c_int32)), ("base", C.c_void_p), ("parent", C.c_void_p)]
+
+
+class GdnConv(C.Structure):
+    """tsv_gdn_conv_io: device addresses, strides in elements."""
+    _fields_ = [("qkv", C.c_void_p), ("qkv_stride", C.c_int64), ("a", C.c_void_p), ("b", C.c_void_p), ("gate_stride", C.c_int64),
+                ("ring", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_int64), ("g", C.c_void_p), ("beta", C.c_void_p)]
+
+
+class GdnPrefill(C.Structure):
+    """tsv_gdn_prefill_io"""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
+                ("v_stride", C.c_int64), ("g", C.c_void_p), ("beta", C.c_void_p), ("z", C.c_void_p), ("z_stride", C.c_int64),
+                ("state_in", C.c_void_p), ("state_out", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_int64),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64)]
+
+
+class GdnStep(C.Structure):
+    """tsv_gdn_step_io"""
+    _fields_ = [("qkv", C.c_void_p), ("qkv_stride", C.c_int64), ("a", C.c_void_p), ("b", C.c_void_p), ("gate_stride", C.c_int64),
+                ("z", C.c_void_p), ("z_stride", C.c_int64), ("ring", C.c_void_p), ("state_in", C.c_void_p), ("state_out", C.c_void_p),
+                ("record", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_int64)]
+
+
+class GdnCommit(C.Structure):
+    """tsv_gdn_commit_io"""
+    _fields_ = [("n_layers", C.c_int32), ("results", C.c_void_p), ("record", C.c_void_p), ("record_stride", C.c_int64),
+                ("ring_in", C.c_void_p), ("ring_out", C.c_void_p), ("ring_stride", C.c_int64), ("state_in", C.c_void_p),
+                ("state_out", C.c_void_p), ("state_stride", C.c_int64)]
+
+
 class Point(C.Structure):
     _fields_ = [("position", C.c_int64)]
 
@@ -261,6 +299,7 @@ EXPORTS = [
     "tsv_session_pool_size", "tsv_session_slot_evicted", "tsv_session_best_match", "tsv_session_lru", "tsv_session_swapped",
     "tsv_kv_row_bytes", "tsv_kv_bytes_for_context",
     "tsv_mtp_open", "tsv_mtp_step", "tsv_mtp_rewind", "tsv_mtp_prefill_chunk", "tsv_mtp_draft_block", "tsv_mtp_drafter",
+    "tsv_gdn_conv", "tsv_gdn_prefill_workspace", "tsv_gdn_prefill", "tsv_gdn_record_bytes", "tsv_gdn_step", "tsv_gdn_commit",
 ]
 
 _lib = None
@@ -349,6 +388,12 @@ def lib():
         L.tsv_mtp_prefill_chunk.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int32]
         L.tsv_mtp_draft_block.argtypes = [C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_void_p]
         L.tsv_mtp_drafter.argtypes = [C.c_void_p, C.POINTER(Drafter)]
+        for name in ("tsv_gdn_conv", "tsv_gdn_prefill", "tsv_gdn_step", "tsv_gdn_commit"):
+            getattr(L, name).argtypes = [C.c_void_p] * 4
+        L.tsv_gdn_prefill_workspace.restype = C.c_int64
+        L.tsv_gdn_prefill_workspace.argtypes = [C.c_void_p, C.c_void_p]
+        L.tsv_gdn_record_bytes.restype = C.c_int64
+        L.tsv_gdn_record_bytes.argtypes = [C.c_void_p, C.c_int64]
         L.tsv_set_profile.argtypes = [C.c_void_p, C.c_int32]
         L.tsv_get_profile.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32]
         L.tsv_copy_time.argtypes = [C.c_int64, C.c_int32, C.POINTER(C.c_float)]
