@@ -467,7 +467,7 @@ int64_t tsv_vocab(const tsv_ctx* ctx);
  * lies in slot p % TSV_GDN_RING, so that nothing has to be erased when a pass is rejected.  A sequence whose base is 0 starts
  * from nothing, whatever its state and ring hold.
  *
- * Rows are bf16 or fp16.  Strides are elements from row to row, multiples of 8; qkv, q, k, v, z, out and the rings are 16-byte
+ * Rows are bf16 or fp16.  Strides are elements from row to row, multiples of 8, at most 2^22; qkv, q, k, v, z, out and the rings are 16-byte
  * aligned.  Rows outside the batch's sequences are neither read nor written.  Outputs must not overlap inputs, but for state_out
  * == state_in and ring_out == ring_in. */
 #define TSV_GDN_RING 32     /* raw rows kept per sequence: conv_width - 1 behind a pass and TSV_MAX_ROWS of it */

@@ -57,6 +57,20 @@ __device__ __forceinline__ void split2(float x, __bf16& hi, __bf16& lo) {
     lo = (__bf16)(x - (float)hi);
 }
 
+// two values at once: bits of (hi of x, hi of y) and of (lo of x, lo of y)
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x, y}), b2));
+    const f2 rest = {x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u)};
+    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, b2));
+}
+__device__ __forceinline__ uint32_t pair_bf16(float x, float y) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x, y}), b2));
+}
+
 __device__ __forceinline__ gf4 mfma_bf16(bf16x8 a, bf16x8 b, gf4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ gf4 mfma_f32(float a, float b, gf4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 

@@ -500,7 +500,7 @@ int gdn_refuse(const char* who, const char* what) {
 }
 
 bool gdn_rows_ok(const void* p, int64_t stride, int64_t width) {
-    return p && ((uintptr_t)p & 15) == 0 && (stride & 7) == 0 && stride >= width && stride <= (int64_t)1 << 40;
+    return p && ((uintptr_t)p & 15) == 0 && (stride & 7) == 0 && stride >= width && stride <= (int64_t)1 << 22;
 }
 
 bool gdn_overlap(const void* a, const void* b, size_t bytes) {

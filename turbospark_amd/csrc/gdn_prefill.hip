@@ -27,11 +27,15 @@ struct PrefillArgs {
     float* state_out;
     uint16_t* out;
     int64_t out_stride;
-    uint4 *kt, *tp;  // workspace: k transposed per (block, key head); T and P fragments per (block, value head)
+    uint4 *kt, *tp;  // workspace: k, q and k transposed per (block, key head); T and P fragments per (block, value head)
     float* gates;    // ... and e^G, e^{G_end - G}
     int32_t tiles;   // column tiles of a head in the walk
     int32_t block_of[TSV_GDN_MAX_SEQ + 1];
 };
+
+// fragments (1 KiB: a wave's 16 bytes a lane) of a (block, key head): k and q by row tile, k transposed by 16 of k_dim
+template <int DK, int TR>
+constexpr int KFRAGS = 4 * (DK / 32) * TR;
 
 __device__ __host__ constexpr int tfrag(int w, int ks) { return w < 2 ? w : 2 * w - 2 + ks; }
 
@@ -77,22 +81,36 @@ __device__ __forceinline__ int sequence_of(const int32_t* starts, int n, int at)
 // value heads, whose decays make A and P of them.  The inverse: each wave inverts its 16 x 16 diagonal block row by row, a column a
 // lane; then wave j does the blocks under diagonal block j, T_ij = -T_ii sum_l A_il T_lj, on the f32 matrix instruction, whose D layout
 // is its B operand's when the contraction takes rows 4 gq + r in step r.
+constexpr int PS = 72;  // row stride (2-byte values) of P in LDS
+// 16-byte units of LDS that hold k's operands, then P
+template <int DK, int TR>
+constexpr int blocks_operands = KFRAGS<DK, TR> * 64 > TR * BLK * PS / 8 ? KFRAGS<DK, TR> * 64 : TR * BLK * PS / 8;
+
 template <int DK, bool F16>
 __global__ __launch_bounds__(256) void k_gdn_blocks(GdnShape sh, GdnBatch bt, PrefillArgs p) {
     constexpr int TR = F16 ? 2 : 1, KS = DK / 32;
     extern __shared__ uint4 lds[];
     uint4* kf = lds;                                   // [row tile][k step][term][lane]
-    float* A = (float*)(kf + 4 * KS * TR * 64);        // [64][MS]
+    uint16_t* P = (uint16_t*)lds;                      // [term][64][PS], where the operands were
+    float* A = (float*)(lds + blocks_operands<DK, TR>);  // [64][MS]
     float* T = A + BLK * MS;
-    float* P = T + BLK * MS;
-    double* G = (double*)(P + BLK * MS);               // [64]
+    double* G = (double*)(T + BLK * MS);               // [64]
     float* be = (float*)(G + BLK);                     // [64]
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, gq = lane >> 4, hk = blockIdx.y;
     const int blk = blockIdx.x, s = sequence_of(p.block_of, bt.n_seq, blk);
     const int r0 = (blk - p.block_of[s]) * BLK, n = min(BLK, bt.off[s + 1] - bt.off[s] - r0);
     const int64_t row0 = bt.off[s] + r0;
     const int mine = 16 * w + l16;
+    float next_g = 0.0f, next_b = 0.0f;
+    auto ask_gates = [&](int h) {
+        if (lane < n) {
+            next_g = p.g[(row0 + lane) * sh.hv + h];
+            next_b = p.beta[(row0 + lane) * sh.hv + h];
+        }
+    };
+    ask_gates(hk * sh.rep);
     bf16x8 kr[KS][TR], qr[KS][TR];
+    uint4* rows_out = p.kt + ((int64_t)blk * sh.hk + hk) * (3 * KFRAGS<DK, TR> * 64);
 #pragma unroll
     for (int t = 0; t < KS; t++) {
         uint4 a = make_uint4(0, 0, 0, 0), b = a;
@@ -103,7 +121,12 @@ __global__ __launch_bounds__(256) void k_gdn_blocks(GdnShape sh, GdnBatch bt, Pr
         row_terms<F16>(a, kr[t]);
         row_terms<F16>(b, qr[t]);
 #pragma unroll
-        for (int e = 0; e < TR; e++) kf[((w * KS + t) * TR + e) * 64 + lane] = __builtin_bit_cast(uint4, kr[t][e]);
+        for (int e = 0; e < TR; e++) {
+            const int f = (w * KS + t) * TR + e;
+            kf[f * 64 + lane] = __builtin_bit_cast(uint4, kr[t][e]);
+            rows_out[f * 64 + lane] = __builtin_bit_cast(uint4, kr[t][e]);
+            rows_out[(KFRAGS<DK, TR> + f) * 64 + lane] = __builtin_bit_cast(uint4, qr[t][e]);
+        }
     }
     __syncthreads();
     gf4 kk[4], qk[4];
@@ -123,7 +146,7 @@ __global__ __launch_bounds__(256) void k_gdn_blocks(GdnShape sh, GdnBatch bt, Pr
     // k transposed, as the operand of the state's update: rows k_dim, eight block rows a lane
     {
         const uint16_t* kh = (const uint16_t*)kf;
-        uint4* to = p.kt + ((int64_t)blk * sh.hk + hk) * (DK / 16 * 2 * TR * 64);
+        uint4* to = rows_out + 2 * KFRAGS<DK, TR> * 64;
         for (int f = w; f < DK / 16 * 2 * TR; f += 4) {
             const int e = f % TR, ks = f / TR % 2, d = 16 * (f / TR / 2) + l16;
             uint16_t x[8];
@@ -136,13 +159,10 @@ __global__ __launch_bounds__(256) void k_gdn_blocks(GdnShape sh, GdnBatch bt, Pr
         }
     }
     for (int h = hk * sh.rep; h < (hk + 1) * sh.rep; h++) {
+        const float b = next_b;
+        const float g = next_g > 0.0f ? 0.0f : next_g < -1e4f ? -1e4f : next_g;  // (e^-1e4 is 0; a sum of infinities has no differences)
+        ask_gates(min(h + 1, (hk + 1) * sh.rep - 1));
         if (w == 0) {
-            float g = 0.0f, b = 0.0f;
-            if (lane < n) {
-                g = p.g[(row0 + lane) * sh.hv + h];
-                b = p.beta[(row0 + lane) * sh.hv + h];
-                g = g > 0.0f ? 0.0f : g < -1e4f ? -1e4f : g;  // (e^-1e4 is 0; a sum of infinities has no differences)
-            }
             double sum = g;
 #pragma unroll
             for (int d = 1; d < 64; d <<= 1) {
@@ -167,7 +187,10 @@ __global__ __launch_bounds__(256) void k_gdn_blocks(GdnShape sh, GdnBatch bt, Pr
                 const int i = 16 * w + 4 * gq + r;
                 const float d = j <= i ? __expf((float)(G[i] - gj)) : 0.0f;
                 A[i * MS + j] = j < i ? be[i] * d * kk[c][r] : 0.0f;
-                P[i * MS + j] = j <= i ? d * qk[c][r] : 0.0f;
+                __bf16 hi, lo;
+                split2(j <= i ? d * qk[c][r] : 0.0f, hi, lo);
+                P[i * PS + j] = __builtin_bit_cast(uint16_t, hi);
+                if constexpr (TR == 2) P[(BLK + i) * PS + j] = __builtin_bit_cast(uint16_t, lo);
             }
         }
         wave_lds_fence();
@@ -221,46 +244,236 @@ __global__ __launch_bounds__(256) void k_gdn_blocks(GdnShape sh, GdnBatch bt, Pr
         for (int ks = 0; ks < 2; ks++) {
             if (ks > w / 2) continue;
             const int f = tfrag(w, ks), j0 = 32 * ks + 8 * gq, row = 16 * w + l16;
-            bf16x8 th, tl, ph, pl;
+            uint4 th, tl;
+            float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const bool in = j0 + e <= row;  // above the diagonal nothing has been written
-                __bf16 hi, lo;
-                split2(in ? T[row * MS + j0 + e] * be[j0 + e] : 0.0f, hi, lo);
-                th[e] = hi;
-                tl[e] = lo;
-                split2(in ? P[row * MS + j0 + e] : 0.0f, hi, lo);
-                ph[e] = hi;
-                pl[e] = lo;
-            }
-            to[(2 * f) * 64 + lane] = __builtin_bit_cast(uint4, th);
-            to[(2 * f + 1) * 64 + lane] = __builtin_bit_cast(uint4, tl);
-            to[(2 * TFRAGS + TR * f) * 64 + lane] = __builtin_bit_cast(uint4, ph);
-            if constexpr (TR == 2) to[(2 * TFRAGS + TR * f + 1) * 64 + lane] = __builtin_bit_cast(uint4, pl);
+            for (int e = 0; e < 8; e++) x[e] = j0 + e <= row ? T[row * MS + j0 + e] * be[j0 + e] : 0.0f;  // above the diagonal nothing has been written
+            split2(x[0], x[1], th.x, tl.x);
+            split2(x[2], x[3], th.y, tl.y);
+            split2(x[4], x[5], th.z, tl.z);
+            split2(x[6], x[7], th.w, tl.w);
+            to[(2 * f) * 64 + lane] = th;
+            to[(2 * f + 1) * 64 + lane] = tl;
+            const bool zero = 32 * ks + 8 * gq >= 16 * (w + 1);  // (columns of row tiles behind this one)
+#pragma unroll
+            for (int e = 0; e < TR; e++) to[(2 * TFRAGS + TR * f + e) * 64 + lane] = zero ? make_uint4(0, 0, 0, 0) : *(const uint4*)(P + (e * BLK + row) * PS + j0);
         }
         __syncthreads();
     }
 }
 
 // ---- the walk through a sequence's blocks --------------------------------------------------------------------------------------------
-// One workgroup of four waves per (sequence, value head, 16 NT value channels).  Wave w owns rows 16 w .. of the block and k_dim / 4
-// rows of the state, which stay in the accumulators; the state, v - e^G kS and u pass between the waves through LDS as bf16 terms in
-// operand order, three barriers a block.  Everything a block reads is asked for one block ahead, into the registers just used.  The
-// column tiles of a head read the same k, q, T and P: workgroups are numbered so that they share an XCD's L2.
+// One workgroup of eight waves per (sequence, value head, 16 NT value channels).  Waves 0 to 3 take the state from block to block:
+// wave w owns rows 16 w .. of the block and k_dim / 4 rows of the state, which stay in its accumulators; the state, v - e^G kS and u
+// pass between them through LDS as bf16 terms in operand order, three barriers a block.  Waves 4 to 7, one beside each of them on a
+// SIMD, make the output rows from the same LDS (q S behind the first barrier, P u behind the third) and hand the others v, transposed,
+// and the decays through LDS: a load or store of any width holds the CU's address unit for 16 cycles, which bounds a block (12 and 9 of
+// them a wave here), so two-byte ones are taken together.  Everything a block reads is asked for one block ahead, into the registers
+// just used: the scheduling fences keep the compiler from asking earlier, which would take copies and, with them, waits.  The column tiles of a head read the same k, q, T and P: workgroups are numbered so that they share an
+// XCD's L2.
+#define GDN_FENCE __builtin_amdgcn_sched_barrier(0)
+// (the wave that brings data into the L2 pays where one workgroup has a compute unit; k_dim 256 needs its registers)
+template <int DK, int NT>
+constexpr int walk_threads = NT == 1 && DK < 256 ? 576 : 512;
+
 template <int DK, bool F16, int NT>
-__global__ __launch_bounds__(256) void k_gdn_walk(GdnShape sh, GdnBatch bt, PrefillArgs p) {
-    constexpr int TR = F16 ? 2 : 1, KS = DK / 32, SD = DK / 64;
+struct Walk {
+    static constexpr int TR = F16 ? 2 : 1, KS = DK / 32, SD = DK / 64;
+    // LDS, all in operand order [k step][nt][term][lane]
+    static constexpr int S_AT = 0, R_AT = KS * NT * 2 * 64, U_AT = R_AT + 2 * NT * 2 * 64, D_AT = U_AT + 2 * NT * TR * 64;
+    // v as [column][VS], the decays e^G and e^{G_end - G}, and the output rows on their way out, a region per wave
+    static constexpr int V_AT = D_AT + 2 * NT * 2 * 64, VS = 72, G_AT = V_AT + 16 * NT * VS / 8, O_AT = G_AT + 32, LDS = O_AT + 64 * 16 * NT / 8;
+    uint4* lds;
+    int lane, w, l16, gq;
+
+    // four consecutive contraction indices of one column, as one or two terms, where the B operand's lane finds its eight
+    template <int TERMS>
+    __device__ __forceinline__ void put(int to, int step, int t, int group, gf4 x) const {
+        uint2* f = (uint2*)(lds + to + (step * NT + t) * TERMS * 64) + (group * 16 + l16) * 2 + (gq & 1);
+        if (TERMS == 2) {
+            uint2 hi, lo;
+            split2(x[0], x[1], hi.x, lo.x);
+            split2(x[2], x[3], hi.y, lo.y);
+            f[0] = hi;
+            f[128] = lo;
+        } else {
+            f[0] = make_uint2(pair_bf16(x[0], x[1]), pair_bf16(x[2], x[3]));
+        }
+    }
+    template <int TERMS>
+    __device__ __forceinline__ void get(int from, int step, int t, bf16x8* x) const {
+#pragma unroll
+        for (int e = 0; e < TERMS; e++) x[e] = __builtin_bit_cast(bf16x8, lds[from + ((step * NT + t) * TERMS + e) * 64 + lane]);
+    }
+};
+
+template <int DK, bool F16, int NT>
+__global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape sh, GdnBatch bt, PrefillArgs p) {
+    typedef Walk<DK, F16, NT> W;
+    constexpr int TR = W::TR, KS = W::KS, SD = W::SD;
     extern __shared__ uint4 lds[];
-    uint4* sf = lds;                        // state: [k step][nt][term][lane]
-    uint4* rf = sf + KS * NT * 2 * 64;      // v - e^G kS: [k step][nt][term][lane]
-    uint4* uf = rf + 2 * NT * 2 * 64;       // u for the output: [k step][nt][term TR][lane]
-    uint4* df = uf + 2 * NT * TR * 64;      // u decayed to the block's end, for the state: [k step][nt][term][lane]
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, gq = lane >> 4;
-    const int y = blockIdx.x >> 3, tile = y % p.tiles, hs = y / p.tiles * 8 + (blockIdx.x & 7);
-    if (hs >= bt.n_seq * sh.hv) return;
-    const int s = hs / sh.hv, h = hs - s * sh.hv, hk = h / sh.rep, first = bt.off[s], rows = bt.off[s + 1] - first;
-    const int blocks = p.block_of[s + 1] - p.block_of[s], col0 = tile * 16 * NT + l16;
-    const size_t at = ((size_t)hs * sh.dv + col0) * DK + 16 * SD * w + 4 * gq;
+    const int tid = threadIdx.x, lane = tid & 63, w8 = __builtin_amdgcn_readfirstlane(tid >> 6), w = w8 & 3, l16 = lane & 15, gq = lane >> 4;
+    const W x{lds, lane, w, l16, gq};
+    // a key head's workgroups, its value heads' column tiles, are 8 apart: the same XCD
+    const int y = blockIdx.x >> 3, of = p.tiles * sh.rep, ks_ = y / of * 8 + (blockIdx.x & 7), tile = y % p.tiles;
+    if (ks_ >= bt.n_seq * sh.hk) return;
+    const int s = ks_ / sh.hk, hk = ks_ - s * sh.hk, h = hk * sh.rep + y % of / p.tiles, hs = s * sh.hv + h, first = bt.off[s], rows = bt.off[s + 1] - first;
+    const int blocks = p.block_of[s + 1] - p.block_of[s];
+    const int64_t b0 = p.block_of[s];
+    // uniform addresses of the block asked for, and what a lane adds to them (in bytes)
+    const char* tpp = (const char*)(p.tp + (b0 * sh.hv + h) * (TFRAGS * (2 + TR) * 64));
+    const char* gp = (const char*)(p.gates + (b0 * sh.hv + h) * 128);
+    const int64_t tp_step = (int64_t)sh.hv * (TFRAGS * (2 + TR) * 1024), g_step = (int64_t)sh.hv * 512;
+    const uint32_t lane16 = lane * 16;
+    // (waves of rows 0 and 16 have one fragment of T and P where the others have two: they ask for theirs twice and clear the copy, so
+    // that every wave has the same loads under way and a wait is for the ones it needs)
+    const uint32_t second = w < 2 ? 0u : 0xFFFFFFFFu;
+    const int f0 = tfrag(w, 0), f1 = w < 2 ? f0 : f0 + 1;
+    auto fragment = [&](const uint4& f, int ks) {
+        if (ks == 0) return __builtin_bit_cast(bf16x8, f);
+        return __builtin_bit_cast(bf16x8, make_uint4(f.x & second, f.y & second, f.z & second, f.w & second));
+    };
+    if (walk_threads<DK, NT> > 512 && w8 == 8) {  // ---- the wave that brings what is four blocks ahead into the XCD's L2, this workgroup's share of it
+        constexpr int AHEAD = 4, LINES = 3 * KFRAGS<DK, TR> * 8 + TFRAGS * (2 + TR) * 8, SHARE = 3;
+        const char* kreg = (const char*)(p.kt + (b0 * sh.hk + hk) * (3 * KFRAGS<DK, TR> * 64));
+        const int64_t k_step = (int64_t)sh.hk * (3 * KFRAGS<DK, TR> * 1024);
+        const char* vreg = (const char*)(p.v + (int64_t)first * p.v_stride + h * sh.dv + tile * 16 * NT);
+        uint32_t got[AHEAD][SHARE + 1] = {};
+        for (int b = 0; b < blocks; b += AHEAD)
+#pragma unroll
+            for (int j = 0; j < AHEAD; j++) {
+                if (b + j >= blocks) break;
+                const int at = min(b + j + AHEAD, blocks - 1);
+#pragma unroll
+                for (int i = 0; i < SHARE + 1; i++) asm volatile("" ::"v"(got[j][i]));  // what was asked for AHEAD blocks ago is there
+#pragma unroll
+                for (int i = 0; i < SHARE; i++) {
+                    const int line = min((i * p.tiles + tile) * 64 + lane, LINES - 1) * 128;
+                    constexpr int KB = 3 * KFRAGS<DK, TR> * 1024;
+                    got[j][i] = *(const uint32_t*)(line < KB ? kreg + at * k_step + line : tpp + at * tp_step + (line - KB));
+                }
+                got[j][SHARE] = *(const uint32_t*)(vreg + (int64_t)min(at * BLK + lane, rows - 1) * (2 * p.v_stride));
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_s_barrier();
+                __builtin_amdgcn_s_barrier();
+            }
+        return;
+    }
+    if (w8 >= 4) {  // ---- the output's waves
+        const char* qp = (const char*)(p.kt + ((b0 * sh.hk + hk) * 3 + 1) * (KFRAGS<DK, TR> * 64) + w * KS * TR * 64);
+        const int64_t q_step = (int64_t)sh.hk * (3 * KFRAGS<DK, TR> * 1024);
+        uint4 qr[KS][TR], pr[2][TR];
+        auto ask_q = [&]() {
+#pragma unroll
+            for (int t = 0; t < KS; t++)
+#pragma unroll
+                for (int e = 0; e < TR; e++) qr[t][e] = *(const uint4*)(qp + (t * TR + e) * 1024 + lane16);
+        };
+        auto ask_p = [&]() {
+#pragma unroll
+            for (int e = 0; e < TR; e++) {
+                pr[0][e] = *(const uint4*)(tpp + (2 * TFRAGS + TR * f0 + e) * 1024 + lane16);
+                pr[1][e] = *(const uint4*)(tpp + (2 * TFRAGS + TR * f1 + e) * 1024 + lane16);
+            }
+        };
+        // a lane's piece of the rows: a quarter of row lane / 4 of the wave's sixteen
+        typedef uint32_t piece __attribute__((ext_vector_type(2 * NT)));
+        const int prow = 16 * w + (lane >> 2), pcol = (lane & 3) * 4 * NT;
+        const uint16_t* vp = p.v + (int64_t)first * p.v_stride + h * sh.dv + tile * 16 * NT + pcol;
+        char* op = (char*)(p.out + (int64_t)first * p.out_stride + h * sh.dv + tile * 16 * NT);
+        const int64_t o_step = p.out_stride * (2 * BLK);
+        const uint32_t o_off = prow * (uint32_t)(2 * p.out_stride) + 2 * pcol;
+        uint16_t* vt = (uint16_t*)(lds + W::V_AT);
+        uint16_t* ot = (uint16_t*)(lds + W::O_AT) + w * 16 * 16 * NT;
+        piece vr;
+        float2 gr;
+        auto ask_v = [&](int b) {  // (rows behind the sequence's last are taken from it: T is 0 there)
+            b = min(b, blocks - 1);
+            vr = *(const piece*)(vp + min(b * BLK + prow, rows - 1) * p.v_stride);
+            if (w == 0) gr = *(const float2*)(gp + b * g_step + 8 * lane);
+        };
+        auto put_v = [&]() {
+#pragma unroll
+            for (int i = 0; i < 2 * NT; i++) {
+                vt[(pcol + 2 * i) * W::VS + prow] = (uint16_t)vr[i];
+                vt[(pcol + 2 * i + 1) * W::VS + prow] = (uint16_t)(vr[i] >> 16);
+            }
+            if (w == 0) ((float2*)(lds + W::G_AT))[lane] = gr;
+        };
+        if (blocks > 0) {
+            ask_v(0);
+            ask_q();
+            ask_p();
+            put_v();
+            ask_v(1);
+        }
+        for (int b = 0; b < blocks; b++) {
+            const bool more = b + 1 < blocks;  // (behind the last block the same one is asked for again)
+            qp += more ? q_step : 0;
+            tpp += more ? tp_step : 0;
+            __syncthreads();
+            bf16x8 st[KS][NT][2];
+#pragma unroll
+            for (int i = 0; i < KS; i++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) x.template get<2>(W::S_AT, i, t, st[i][t]);
+            const gf4 eg = *(const gf4*)((const float*)(lds + W::G_AT) + 16 * w + 4 * gq);
+            GDN_FENCE;
+            gf4 o[NT], o2[NT];
+#pragma unroll
+            for (int t = 0; t < NT; t++) o[t] = o2[t] = gf4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < KS; i++) {
+                bf16x8 a[TR];
+#pragma unroll
+                for (int e = 0; e < TR; e++) a[e] = __builtin_bit_cast(bf16x8, qr[i][e]);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    o[t] = mfma_bf16(a[0], st[i][t][0], o[t]);
+                    o2[t] = mfma_bf16(a[0], st[i][t][1], o2[t]);
+                    if constexpr (TR == 2) o2[t] = mfma_bf16(a[1], st[i][t][0], o2[t]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++) o[t] = (o[t] + o2[t]) * eg;
+            GDN_FENCE;
+            __syncthreads();
+            ask_q();
+            __syncthreads();
+            bf16x8 u[2][NT][TR];
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) x.template get<TR>(W::U_AT, ks, t, u[ks][t]);
+            put_v();  // (the others are done with this block's)
+            GDN_FENCE;
+            ask_v(b + 2);
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+                bf16x8 a[TR];
+#pragma unroll
+                for (int e = 0; e < TR; e++) a[e] = fragment(pr[ks][e], ks);
+#pragma unroll
+                for (int t = 0; t < NT; t++) o[t] = mfma_terms<TR, TR>(a, u[ks][t], o[t]);
+            }
+            GDN_FENCE;
+            ask_p();
+#pragma unroll
+            for (int t = 0; t < NT; t++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) ot[(4 * gq + r) * 16 * NT + 16 * t + l16] = row_bits<F16>(sh.scale * o[t][r]);
+            wave_lds_fence();
+            const piece out = *(const piece*)(ot + (lane >> 2) * 16 * NT + pcol);
+            // (a buffer's end at the sequence's last row: stores behind it are dropped by the hardware, without a branch)
+            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(op, 0, ((uint32_t)min(rows - b * BLK, BLK) - 1) * (uint32_t)(2 * p.out_stride) + 32 * NT, 0x00027000);
+            if constexpr (NT == 1) __builtin_amdgcn_raw_buffer_store_b64(out, rsrc, o_off, 0, 0);
+            else __builtin_amdgcn_raw_buffer_store_b128(out, rsrc, o_off, 0, 0);
+            op += o_step;
+        }
+        return;
+    }
+    // ---- the state's waves
+    const size_t at = ((size_t)hs * sh.dv + tile * 16 * NT + l16) * DK + 16 * SD * w + 4 * gq;
     const bool fresh = bt.base[s] == 0;
     gf4 S[SD][NT];
 #pragma unroll
@@ -270,193 +483,151 @@ __global__ __launch_bounds__(256) void k_gdn_walk(GdnShape sh, GdnBatch bt, Pref
             S[d][t] = *(const gf4*)(p.state_in + at + (size_t)16 * t * DK + 16 * d);
             if (fresh) S[d][t] = gf4{0, 0, 0, 0};
         }
-    const uint16_t* kp = p.k + (int64_t)first * p.k_stride + hk * DK + 8 * gq;
-    const uint16_t* qp = p.q + (int64_t)first * p.q_stride + hk * DK + 8 * gq;
-    const uint16_t* vp = p.v + (int64_t)first * p.v_stride + h * sh.dv + col0;
-    const int64_t b0 = p.block_of[s];
-    const uint4* ktp = p.kt + (b0 * sh.hk + hk) * (DK / 16 * 2 * TR * 64) + SD * w * 2 * TR * 64 + lane;
-    const uint4* tpp = p.tp + (b0 * sh.hv + h) * (TFRAGS * (2 + TR) * 64) + lane;
-    const float* gp = p.gates + (b0 * sh.hv + h) * 128 + 16 * w + 4 * gq;
-    const int64_t kt_step = (int64_t)sh.hk * (DK / 16 * 2 * TR * 64), tp_step = (int64_t)sh.hv * (TFRAGS * (2 + TR) * 64), g_step = (int64_t)sh.hv * 128;
-    const int nks = w / 2 + 1, f0 = tfrag(w, 0);
-
-    uint4 kr[KS], qr[KS], ktr[SD][2][TR], tr[2][2], pr[2][TR];
-    uint16_t vr[NT][4];
-    gf4 eg, ed;
-    float e_end;
-    auto ask_kq = [&](int b) {
-        const int row = min(b * BLK + 16 * w + l16, rows - 1);  // (rows behind the sequence's last: T and k transposed are 0 there)
+    const char* kp = (const char*)(p.kt + (b0 * sh.hk + hk) * (3 * KFRAGS<DK, TR> * 64) + w * KS * TR * 64);
+    const char* ktp = (const char*)(p.kt + ((b0 * sh.hk + hk) * 3 + 2) * (KFRAGS<DK, TR> * 64) + SD * w * 2 * TR * 64);
+    const int64_t k_step = (int64_t)sh.hk * (3 * KFRAGS<DK, TR> * 1024);
+    uint4 kr[KS][TR], ktr[SD][2][TR], tr[2][2];
+    const uint16_t* vt = (const uint16_t*)(lds + W::V_AT) + l16 * W::VS + 16 * w + 4 * gq;
+    const float* gates = (const float*)(lds + W::G_AT);
+    auto ask_k = [&]() {
 #pragma unroll
-        for (int t = 0; t < KS; t++) kr[t] = *(const uint4*)(kp + row * p.k_stride + 32 * t);
+        for (int t = 0; t < KS; t++)
 #pragma unroll
-        for (int t = 0; t < KS; t++) qr[t] = *(const uint4*)(qp + row * p.q_stride + 32 * t);
+            for (int e = 0; e < TR; e++) kr[t][e] = *(const uint4*)(kp + (t * TR + e) * 1024 + lane16);
     };
-    auto ask_v = [&](int b) {
+    auto ask_t = [&]() {
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int row = min(b * BLK + 16 * w + 4 * gq + r, rows - 1);
-#pragma unroll
-            for (int t = 0; t < NT; t++) vr[t][r] = vp[row * p.v_stride + 16 * t];
+        for (int e = 0; e < 2; e++) {
+            tr[0][e] = *(const uint4*)(tpp + (2 * f0 + e) * 1024 + lane16);
+            tr[1][e] = *(const uint4*)(tpp + (2 * f1 + e) * 1024 + lane16);
         }
-        eg = *(const gf4*)(gp + b * g_step);
     };
-    auto ask_t = [&](int b) {
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++)
-            if (ks < nks) {
-#pragma unroll
-                for (int e = 0; e < 2; e++) tr[ks][e] = tpp[b * tp_step + (2 * (f0 + ks) + e) * 64];
-            }
-        ed = *(const gf4*)(gp + b * g_step + 64);
-    };
-    auto ask_kt = [&](int b) {
+    auto ask_kt = [&]() {
 #pragma unroll
         for (int d = 0; d < SD; d++)
 #pragma unroll
             for (int ks = 0; ks < 2; ks++)
 #pragma unroll
-                for (int e = 0; e < TR; e++) ktr[d][ks][e] = ktp[b * kt_step + ((d * 2 + ks) * TR + e) * 64];
-        e_end = p.gates[((b0 + b) * sh.hv + h) * 128 + 63];
-    };
-    auto ask_p = [&](int b) {
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++)
-            if (ks < nks) {
-#pragma unroll
-                for (int e = 0; e < TR; e++) pr[ks][e] = tpp[b * tp_step + (2 * TFRAGS + TR * (f0 + ks) + e) * 64];
-            }
-    };
-    // four consecutive contraction indices of one column, as two terms, where the B operand's lane finds its eight
-    auto put = [&](uint4* to, int step, int t, int terms, int group, float x0, float x1, float x2, float x3) {
-        const float x[4] = {x0, x1, x2, x3};
-        __bf16 hi[4], lo[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) split2(x[i], hi[i], lo[i]);
-        uint2* f = (uint2*)(to + (step * NT + t) * terms * 64) + (group * 16 + l16) * 2 + (gq & 1);
-        f[0] = *(uint2*)hi;
-        if (terms == 2) f[128] = *(uint2*)lo;
-    };
-    auto get = [&](const uint4* from, int step, int t, int terms, bf16x8* x) {
-#pragma unroll
-        for (int e = 0; e < terms; e++) x[e] = __builtin_bit_cast(bf16x8, from[((step * NT + t) * terms + e) * 64 + lane]);
+                for (int e = 0; e < TR; e++) ktr[d][ks][e] = *(const uint4*)(ktp + ((d * 2 + ks) * TR + e) * 1024 + lane16);
     };
     auto put_state = [&]() {
 #pragma unroll
-        for (int d = 0; d < SD; d++) {
-            const int tile16 = SD * w + d;
+        for (int d = 0; d < SD; d++)
 #pragma unroll
-            for (int t = 0; t < NT; t++) put(sf, tile16 >> 1, t, 2, 2 * (tile16 & 1) + (gq >> 1), S[d][t][0], S[d][t][1], S[d][t][2], S[d][t][3]);
-        }
+            for (int t = 0; t < NT; t++) x.template put<2>(W::S_AT, (SD * w + d) >> 1, t, 2 * ((SD * w + d) & 1) + (gq >> 1), S[d][t]);
     };
     if (blocks > 0) {
-        ask_kq(0);
-        ask_v(0);
-        ask_t(0);
-        ask_kt(0);
-        ask_p(0);
+        ask_k();
+        ask_t();
+        ask_kt();
         put_state();
     }
     for (int b = 0; b < blocks; b++) {
-        const int next = min(b + 1, blocks - 1);
+        const bool more = b + 1 < blocks;
+        kp += more ? k_step : 0;
+        ktp += more ? k_step : 0;
+        tpp += more ? tp_step : 0;
         __syncthreads();
-        gf4 ks_[NT], o[NT];
+        {
+            bf16x8 st[KS][NT][2];
 #pragma unroll
-        for (int t = 0; t < NT; t++) ks_[t] = o[t] = gf4{0, 0, 0, 0};
+            for (int i = 0; i < KS; i++)
 #pragma unroll
-        for (int i = 0; i < KS; i++) {
-            bf16x8 kt_[TR], qt_[TR];
-            row_terms<F16>(kr[i], kt_);
-            row_terms<F16>(qr[i], qt_);
+                for (int t = 0; t < NT; t++) x.template get<2>(W::S_AT, i, t, st[i][t]);
+            uint2 v4[NT];
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                bf16x8 x[2];
-                get(sf, i, t, 2, x);
-                ks_[t] = mfma_terms<TR, 2>(kt_, x, ks_[t]);
-                o[t] = mfma_terms<TR, 2>(qt_, x, o[t]);
-            }
-        }
-        ask_kq(next);
+            for (int t = 0; t < NT; t++) v4[t] = *(const uint2*)(vt + 16 * t * W::VS);
+            const gf4 eg = *(const gf4*)(gates + 16 * w + 4 * gq);
+            GDN_FENCE;
+            gf4 c[NT], c2[NT];
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            float x[4];
+            for (int t = 0; t < NT; t++) c[t] = c2[t] = gf4{0, 0, 0, 0};
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                x[r] = fmaf(-eg[r], ks_[t][r], row_f32<F16>(vr[t][r]));
-                o[t][r] *= eg[r];
-            }
-            put(rf, w >> 1, t, 2, 2 * (w & 1) + (gq >> 1), x[0], x[1], x[2], x[3]);
-        }
-        ask_v(next);
-        __syncthreads();
-        gf4 u[NT];
-#pragma unroll
-        for (int t = 0; t < NT; t++) u[t] = gf4{0, 0, 0, 0};
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++)
-            if (ks < nks) {
-                const bf16x8 a[2] = {__builtin_bit_cast(bf16x8, tr[ks][0]), __builtin_bit_cast(bf16x8, tr[ks][1])};
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    bf16x8 x[2];
-                    get(rf, ks, t, 2, x);
-                    u[t] = mfma_terms<2, 2>(a, x, u[t]);
-                }
-            }
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            put(uf, w >> 1, t, TR, 2 * (w & 1) + (gq >> 1), u[t][0], u[t][1], u[t][2], u[t][3]);
-            put(df, w >> 1, t, 2, 2 * (w & 1) + (gq >> 1), ed[0] * u[t][0], ed[1] * u[t][1], ed[2] * u[t][2], ed[3] * u[t][3]);
-        }
-        ask_t(next);
-        __syncthreads();
-#pragma unroll
-        for (int d = 0; d < SD; d++)
-#pragma unroll
-            for (int t = 0; t < NT; t++) S[d][t] *= e_end;
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++)
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                bf16x8 x[2];
-                get(df, ks, t, 2, x);
-#pragma unroll
-                for (int d = 0; d < SD; d++) {
-                    bf16x8 a[TR];
-#pragma unroll
-                    for (int e = 0; e < TR; e++) a[e] = __builtin_bit_cast(bf16x8, ktr[d][ks][e]);
-                    S[d][t] = mfma_terms<TR, 2>(a, x, S[d][t]);
-                }
-            }
-        ask_kt(next);
-        put_state();
-#pragma unroll
-        for (int ks = 0; ks < 2; ks++)
-            if (ks < nks) {
+            for (int i = 0; i < KS; i++) {
                 bf16x8 a[TR];
 #pragma unroll
-                for (int e = 0; e < TR; e++) a[e] = __builtin_bit_cast(bf16x8, pr[ks][e]);
+                for (int e = 0; e < TR; e++) a[e] = __builtin_bit_cast(bf16x8, kr[i][e]);
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
-                    bf16x8 x[TR];
-                    get(uf, ks, t, TR, x);
-                    o[t] = mfma_terms<TR, TR>(a, x, o[t]);
+                    c[t] = mfma_bf16(a[0], st[i][t][0], c[t]);
+                    c2[t] = mfma_bf16(a[0], st[i][t][1], c2[t]);
+                    if constexpr (TR == 2) c2[t] = mfma_bf16(a[1], st[i][t][0], c2[t]);
                 }
             }
-        ask_p(next);
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-            const int row = b * BLK + 16 * w + 4 * gq + r;
-            if (row < rows) {
+            for (int t = 0; t < NT; t++) {
+                gf4 d;
 #pragma unroll
-                for (int t = 0; t < NT; t++) p.out[(int64_t)(first + row) * p.out_stride + h * sh.dv + col0 + 16 * t] = row_bits<F16>(sh.scale * o[t][r]);
+                for (int r = 0; r < 4; r++) d[r] = fmaf(-eg[r], c[t][r] + c2[t][r], row_f32<F16>((uint16_t)((r & 2 ? v4[t].y : v4[t].x) >> (16 * (r & 1)))));
+                x.template put<2>(W::R_AT, w >> 1, t, 2 * (w & 1) + (gq >> 1), d);
             }
         }
+        __syncthreads();
+        {
+            bf16x8 d[2][NT][2];
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) x.template get<2>(W::R_AT, ks, t, d[ks][t]);
+            GDN_FENCE;
+            const gf4 ed = *(const gf4*)(gates + 64 + 16 * w + 4 * gq);
+            const float e_end = gates[63];
+            ask_k();
+            GDN_FENCE;
+            gf4 u[NT], u2[NT];
+#pragma unroll
+            for (int t = 0; t < NT; t++) u[t] = u2[t] = gf4{0, 0, 0, 0};
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++) {
+                const bf16x8 a0 = fragment(tr[ks][0], ks), a1 = fragment(tr[ks][1], ks);
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    u[t] = mfma_bf16(a0, d[ks][t][0], u[t]);
+                    u2[t] = mfma_bf16(a0, d[ks][t][1], u2[t]);
+                    u2[t] = mfma_bf16(a1, d[ks][t][0], u2[t]);
+                }
+            }
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                u[t] += u2[t];
+                x.template put<2>(W::D_AT, w >> 1, t, 2 * (w & 1) + (gq >> 1), ed * u[t]);
+                x.template put<TR>(W::U_AT, w >> 1, t, 2 * (w & 1) + (gq >> 1), u[t]);
+            }
+#pragma unroll
+            for (int i = 0; i < SD; i++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) S[i][t] *= e_end;
+        }
+        __syncthreads();
+        {
+            bf16x8 d[2][NT][2];
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+                for (int t = 0; t < NT; t++) x.template get<2>(W::D_AT, ks, t, d[ks][t]);
+            GDN_FENCE;
+            ask_t();
+            GDN_FENCE;
+#pragma unroll
+            for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+                for (int i = 0; i < SD; i++) {
+                    bf16x8 a[TR];
+#pragma unroll
+                    for (int e = 0; e < TR; e++) a[e] = __builtin_bit_cast(bf16x8, ktr[i][ks][e]);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) S[i][t] = mfma_terms<TR, 2>(a, d[ks][t], S[i][t]);
+                }
+        }
+        ask_kt();
+        put_state();
     }
 #pragma unroll
     for (int d = 0; d < SD; d++)
 #pragma unroll
         for (int t = 0; t < NT; t++) *(gf4*)(p.state_out + at + (size_t)16 * t * DK + 16 * d) = S[d][t];
 }
+#undef GDN_FENCE
 
 // ---- the gated norm, in place --------------------------------------------------------------------------------------------------------
 // v_dim / 8 of GROUP neighbouring lanes hold a head's row.
@@ -493,7 +664,7 @@ struct Sizes {
 Sizes workspace_of(const GdnShape& sh, int dk, bool f16, int64_t blocks) {
     const int tr = f16 ? 2 : 1;
     Sizes z;
-    z.kt = blocks * sh.hk * (dk / 16 * 2 * tr * 1024);
+    z.kt = blocks * sh.hk * (3 * (dk / 8) * tr * 1024);
     z.tp = blocks * sh.hv * (TFRAGS * (2 + tr) * 1024);
     z.gates = blocks * sh.hv * 512;
     z.total = z.kt + z.tp + z.gates;
@@ -509,7 +680,7 @@ int64_t blocks_of(const GdnBatch& bt) {
 template <int DK, bool F16>
 int launch_blocks(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const PrefillArgs& p, int blocks) {
     constexpr int TR = F16 ? 2 : 1;
-    const size_t lds = (size_t)4 * (DK / 32) * TR * 1024 + 3 * BLK * MS * 4 + BLK * 12;
+    const size_t lds = (size_t)blocks_operands<DK, TR> * 16 + 2 * BLK * MS * 4 + BLK * 12;
     static OncePerDevice once;
     const int rc = allow_lds((const void*)k_gdn_blocks<DK, F16>, lds, once);
     if (rc) return rc;
@@ -520,14 +691,13 @@ int launch_blocks(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const 
 
 template <int DK, bool F16, int NT>
 int launch_walk(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, PrefillArgs& p) {
-    constexpr int TR = F16 ? 2 : 1;
-    const size_t lds = (size_t)(DK / 32 * 2 + 2 * 2 + 2 * TR + 2 * 2) * NT * 1024;
+    const size_t lds = (size_t)Walk<DK, F16, NT>::LDS * 16;
     static OncePerDevice once;
     const int rc = allow_lds((const void*)k_gdn_walk<DK, F16, NT>, lds, once);
     if (rc) return rc;
     p.tiles = sh.dv / (16 * NT);
-    const int heads = bt.n_seq * sh.hv;
-    hipLaunchKernelGGL((k_gdn_walk<DK, F16, NT>), dim3((heads + 7) / 8 * 8 * p.tiles), dim3(256), lds, st, sh, bt, p);
+    const int heads = bt.n_seq * sh.hk;
+    hipLaunchKernelGGL((k_gdn_walk<DK, F16, NT>), dim3((heads + 7) / 8 * 8 * sh.rep * p.tiles), dim3(walk_threads<DK, NT>), lds, st, sh, bt, p);
     TSV_HIP(hipGetLastError());
     return TSV_OK;
 }
@@ -538,7 +708,11 @@ int launch_prefill(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, Prefi
         const int rc = launch_blocks<DK, F16>(st, sh, bt, p, blocks);
         if (rc) return rc;
     }
-    if (sh.dv % 32 == 0) return launch_walk<DK, F16, 2>(st, sh, bt, p);
+    // Two column tiles a workgroup where that still gives every compute unit one: they share what a block reads (6 sequences, 32 heads of
+    // 128: 70 us against 100); else one, for the shorter way through a block (8192 rows, 32 heads: 189 us against 219).  k_dim 256 has no
+    // registers for two.
+    if constexpr (DK < 256)
+        if (sh.dv % 32 == 0 && (int64_t)bt.n_seq * sh.hv * (sh.dv / 32) >= 256) return launch_walk<DK, F16, 2>(st, sh, bt, p);
     return launch_walk<DK, F16, 1>(st, sh, bt, p);
 }
 
