@@ -41,6 +41,17 @@ __device__ __forceinline__ uint16_t row_bits(float x) {
     return __builtin_bit_cast(uint16_t, (__bf16)x);
 }
 template <bool F16>
+__device__ __forceinline__ uint32_t row_pair(float x, float y) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    if constexpr (F16) {
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x, y}), h2));
+    } else {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x, y}), b2));
+    }
+}
+template <bool F16>
 __device__ __forceinline__ void row8_f32(const uint4& u, float* x) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -59,16 +70,8 @@ __device__ __forceinline__ void split2(float x, __bf16& hi, __bf16& lo) {
 
 // two values at once: bits of (hi of x, hi of y) and of (lo of x, lo of y)
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    hi = __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x, y}), b2));
-    const f2 rest = {x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u)};
-    lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(rest, b2));
-}
-__device__ __forceinline__ uint32_t pair_bf16(float x, float y) {
-    typedef float f2 __attribute__((ext_vector_type(2)));
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{x, y}), b2));
+    hi = row_pair<false>(x, y);
+    lo = row_pair<false>(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u));
 }
 
 __device__ __forceinline__ gf4 mfma_bf16(bf16x8 a, bf16x8 b, gf4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
@@ -78,6 +81,17 @@ __device__ __forceinline__ float silu_f32(float x) { return x * __builtin_amdgcn
 __device__ __forceinline__ float sigmoid_f32(float x) { return 1.0f / (1.0f + expf(-x)); }
 __device__ __forceinline__ float decay_of(float a_log, float x) {
     return -expf(a_log) * (fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
+}
+
+// The sum of x over LANES neighbouring lanes (8, 16 or 32), in all of them: lanes 1, 2, 7 - i and 15 - i apart, without LDS.
+template <int LANES>
+__device__ __forceinline__ float sum_lanes(float x) {
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xF, 0xF, true));   // quad_perm 1 0 3 2
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xF, 0xF, true));   // quad_perm 2 3 0 1
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xF, 0xF, true));  // row_half_mirror
+    if constexpr (LANES >= 16) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xF, 0xF, true));  // row_mirror
+    if constexpr (LANES >= 32) x += __shfl_xor(x, 16);
+    return x;
 }
 
 // orders a wave's own LDS writes before its own later reads, where no other wave is involved

@@ -8,10 +8,11 @@
 namespace tsv {
 
 // ---- the short convolution of prompt rows ---------------------------------------------------------------------------------
-// A thread owns 8 neighbouring channels and walks CONV_ROWS rows of them with the taps' rows in registers, so that every row is
-// read once (and conv_width - 1 of them again per tile); the k_dim / 8 threads of a head are neighbours in a wave and sum its
-// squares by lane exchange.  Bound by memory: 4 bytes a channel.
-constexpr int CONV_ROWS = 16, CONV_THREADS = 256;
+// A thread owns 8 neighbouring channels and walks a tile of rows, four at a time with the next four under way and the taps' rows in
+// registers: every row is read once, conv_width - 1 of them again per tile.  The k_dim / 8 threads of a head are neighbours in a wave
+// and sum its squares by lane moves.  Bound by memory (4 bytes a channel) and, close behind, by the exponential and the reciprocal of
+// each SiLU.  Tiles have 32 rows, or 4 where 32 would leave compute units without a workgroup.
+constexpr int CONV_THREADS = 256;
 
 struct ConvArgs {
     const uint16_t* qkv;
@@ -23,7 +24,7 @@ struct ConvArgs {
     int64_t out_stride;
     float *g, *beta;
     int32_t tile_of[TSV_GDN_MAX_SEQ + 1];  // first row tile of every sequence
-    int32_t channel_blocks;
+    int32_t channel_blocks, tile_rows;
 };
 
 template <int DK, bool F16>
@@ -34,9 +35,8 @@ __global__ __launch_bounds__(CONV_THREADS) void k_gdn_conv(GdnShape sh, GdnBatch
         if (p.tile_of[mid] <= (int)blockIdx.x) lo = mid;
         else hi = mid;
     }
-    const int s = lo, first = bt.off[s], n = bt.off[s + 1] - first, r0 = ((int)blockIdx.x - p.tile_of[s]) * CONV_ROWS;
-    const int rows = min(CONV_ROWS, n - r0);
-    const int64_t base = bt.base[s];
+    const int s = lo, first = bt.off[s], n = bt.off[s + 1] - first, r0 = ((int)blockIdx.x - p.tile_of[s]) * p.tile_rows;
+    const int rows = min(p.tile_rows, n - r0);
     if ((int)blockIdx.y == p.channel_blocks) {  // the gates' block
         for (int i = threadIdx.x; i < rows * sh.hv; i += CONV_THREADS) {
             const int r = i / sh.hv, h = i - r * sh.hv;
@@ -49,51 +49,68 @@ __global__ __launch_bounds__(CONV_THREADS) void k_gdn_conv(GdnShape sh, GdnBatch
     const int c = ((int)blockIdx.y * CONV_THREADS + threadIdx.x) * 8;
     if (c >= sh.channels) return;  // (a head's threads stay or leave together: head widths are multiples of 16 channels)
     const int taps = sh.taps;
-    float w[4][8], x[4][8];
+    const uint16_t* in = p.qkv + (int64_t)(first + r0) * p.qkv_stride + c;
+    uint16_t* out = p.out + (int64_t)(first + r0) * p.out_stride + c;
+    uint4 ahead[4];
 #pragma unroll
-    for (int j = 0; j < 4; j++)
+    for (int r = 0; r < 4; r++) ahead[r] = *(const uint4*)(in + min(r, rows - 1) * p.qkv_stride);
+    float w[4][8], x[7][8];  // w[j]: j rows back; x[3 - j]: the row j before the four in hand
+    if (taps == 4) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) w[j][e] = j < taps ? sh.conv[(int64_t)(c + e) * taps + taps - 1 - j] : 0.0f;  // w[j]: j rows back
+        for (int e = 0; e < 8; e++) {
+            const uf4 t = *(const uf4*)(sh.conv + (int64_t)(c + e) * 4);
+#pragma unroll
+            for (int j = 0; j < 4; j++) w[j][e] = t[3 - j];
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[j][e] = j < taps ? sh.conv[(int64_t)(c + e) * taps + taps - 1 - j] : 0.0f;
+    }
     uint16_t* ring = p.ring + (int64_t)s * TSV_GDN_RING * sh.channels + c;
+    const int64_t base = r0 == 0 ? bt.base[s] : 0;
 #pragma unroll
     for (int j = 1; j < 4; j++) {
         uint4 u = make_uint4(0, 0, 0, 0);
         if (j < taps) {
-            if (r0 - j >= 0) u = *(const uint4*)(p.qkv + (int64_t)(first + r0 - j) * p.qkv_stride + c);
-            else if (base + r0 - j >= 0) u = *(const uint4*)(ring + ((base + r0 - j) & (TSV_GDN_RING - 1)) * sh.channels);
+            if (r0 - j >= 0) u = *(const uint4*)(in - j * p.qkv_stride);
+            else if (base - j >= 0) u = *(const uint4*)(ring + ((base - j) & (TSV_GDN_RING - 1)) * sh.channels);
         }
-        row8_f32<F16>(u, x[j]);
+        row8_f32<F16>(u, x[3 - j]);
     }
     const bool unit = c < 2 * sh.hk * DK;
-    for (int r = 0; r < rows; r++) {
-        const int64_t row = first + r0 + r;
-        row8_f32<F16>(*(const uint4*)(p.qkv + row * p.qkv_stride + c), x[0]);
-        float y[8], sum = 0.0f;
+    for (int r = 0; r < rows; r += 4) {
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            float v = x[0][e] * w[0][e];
+        for (int i = 0; i < 4; i++) row8_f32<F16>(ahead[i], x[3 + i]);
+        if (r + 4 < rows) {
 #pragma unroll
-            for (int j = 1; j < 4; j++) v = fmaf(x[j][e], w[j][e], v);
-            y[e] = silu_f32(v);
-            sum = fmaf(y[e], y[e], sum);
+            for (int i = 0; i < 4; i++) ahead[i] = *(const uint4*)(in + min(r + 4 + i, rows - 1) * p.qkv_stride);
         }
-        if (unit) {
 #pragma unroll
-            for (int d = 1; d < DK / 8; d <<= 1) sum += __shfl_xor(sum, d);
-            const float f = rsqrtf(sum + sh.l2_eps);
+        for (int i = 0; i < 4; i++) {
+            float y[8], sum = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[e] *= f;
+            for (int e = 0; e < 8; e++) {
+                float v = x[3 + i][e] * w[0][e];
+#pragma unroll
+                for (int j = 1; j < 4; j++) v = fmaf(x[3 + i - j][e], w[j][e], v);
+                y[e] = silu_f32(v);
+            }
+            if (unit) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) sum = fmaf(y[e], y[e], sum);
+                const float f = rsqrtf(sum_lanes<DK / 8>(sum) + sh.l2_eps);
+#pragma unroll
+                for (int e = 0; e < 8; e++) y[e] *= f;
+            }
+            if (r + i < rows)
+                *(uint4*)(out + (r + i) * p.out_stride) = make_uint4(row_pair<F16>(y[0], y[1]), row_pair<F16>(y[2], y[3]), row_pair<F16>(y[4], y[5]), row_pair<F16>(y[6], y[7]));
         }
-        uint4 o;
-        o.x = row_bits<F16>(y[0]) | (uint32_t)row_bits<F16>(y[1]) << 16;
-        o.y = row_bits<F16>(y[2]) | (uint32_t)row_bits<F16>(y[3]) << 16;
-        o.z = row_bits<F16>(y[4]) | (uint32_t)row_bits<F16>(y[5]) << 16;
-        o.w = row_bits<F16>(y[6]) | (uint32_t)row_bits<F16>(y[7]) << 16;
-        *(uint4*)(p.out + row * p.out_stride + c) = o;
 #pragma unroll
-        for (int j = 3; j > 0; j--)
+        for (int j = 0; j < 3; j++)
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[j][e] = x[j - 1][e];
+            for (int e = 0; e < 8; e++) x[j][e] = x[4 + j][e];
     }
     // the ring's new rows, by the thread that has read the old ones of these channels
     if (r0 == 0)
@@ -627,8 +644,9 @@ extern "C" int32_t tsv_gdn_conv(void* stream, const tsv_gdn_layer* layer, const 
     p.g = io->g;
     p.beta = io->beta;
     p.tile_of[0] = 0;
-    for (int s = 0; s < bt.n_seq; s++) p.tile_of[s + 1] = p.tile_of[s] + (bt.off[s + 1] - bt.off[s] + CONV_ROWS - 1) / CONV_ROWS;
     p.channel_blocks = (sh.channels / 8 + CONV_THREADS - 1) / CONV_THREADS;
+    p.tile_rows = (int64_t)bt.off[bt.n_seq] * p.channel_blocks >= 32 * 512 ? 32 : 4;
+    for (int s = 0; s < bt.n_seq; s++) p.tile_of[s + 1] = p.tile_of[s] + (bt.off[s + 1] - bt.off[s] + p.tile_rows - 1) / p.tile_rows;
     const int tiles = p.tile_of[bt.n_seq];
     if (!tiles) return TSV_OK;
     const hipStream_t st = (hipStream_t)stream;

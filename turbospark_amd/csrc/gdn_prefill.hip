@@ -297,7 +297,7 @@ struct Walk {
             f[0] = hi;
             f[128] = lo;
         } else {
-            f[0] = make_uint2(pair_bf16(x[0], x[1]), pair_bf16(x[2], x[3]));
+            f[0] = make_uint2(row_pair<false>(x[0], x[1]), row_pair<false>(x[2], x[3]));
         }
     }
     template <int TERMS>
