@@ -78,9 +78,18 @@ __device__ __forceinline__ gf4 mfma_bf16(bf16x8 a, bf16x8 b, gf4 c) { return __b
 __device__ __forceinline__ gf4 mfma_f32(float a, float b, gf4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
 __device__ __forceinline__ float silu_f32(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
-__device__ __forceinline__ float sigmoid_f32(float x) { return 1.0f / (1.0f + expf(-x)); }
+__device__ __forceinline__ float sigmoid_f32(float x) { return __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
+// g = -e^a_log softplus(x), softplus(x) = max(x, 0) + log(1 + e^-|x|); log(1 + t) = 2 artanh(t / (2 + t)), whose series at t / (2 + t)
+// <= 1/3 is 2^-24 off behind its seventh term: small t keep their bits and the code stays short
 __device__ __forceinline__ float decay_of(float a_log, float x) {
-    return -expf(a_log) * (fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
+    const float t = __expf(-fabsf(x)), s = t * __builtin_amdgcn_rcpf(2.0f + t), q = s * s;
+    float y = fmaf(q, 1.0f / 13.0f, 1.0f / 11.0f);
+    y = fmaf(q, y, 1.0f / 9.0f);
+    y = fmaf(q, y, 1.0f / 7.0f);
+    y = fmaf(q, y, 1.0f / 5.0f);
+    y = fmaf(q, y, 1.0f / 3.0f);
+    y = fmaf(q, y, 1.0f);
+    return -__expf(a_log) * fmaf(2.0f * s, y, fmaxf(x, 0.0f));
 }
 
 // The sum of x over LANES neighbouring lanes (8, 16 or 32), in all of them: lanes 1, 2, 7 - i and 15 - i apart, without LDS.

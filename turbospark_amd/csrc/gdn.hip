@@ -120,13 +120,14 @@ __global__ __launch_bounds__(CONV_THREADS) void k_gdn_conv(GdnShape sh, GdnBatch
 
 // ---- the step of a few rows -------------------------------------------------------------------------------------------------
 // One workgroup per (value head, sequence), a wave per 16 value channels.  A wave's part of the state (16 x k_dim f32) is asked
-// for first and stays in registers; what the rows need beside it is made meanwhile: the convolution of the head's q, k and v
-// channels, the unit vectors as two bf16 terms in operand order, D_ij = exp(sum of g from j, exclusive, to i) along the root
-// paths, and from D and the products k_i.k_j, q_i.k_j the 16 x 16 matrices
-//     T = (I + A)^-1,  A_ij = beta_i D_ij k_i.k_j (j a strict ancestor of i),    P_ij = D_ij q_i.k_j (j an ancestor or i).
-// Then, for all rows at once: KS = k S, QS = q S (three bf16 products each: 2^-17, see split2), u = T beta (v - e^G KS),
-// o = e^G QS + P u, and for final rows S <- e^G_end S + sum_i D_end,i k_i u_i (f32 matrix instructions).  With many sequences the
-// state's bytes bound it, with one the chain of loads and barriers.
+// for first and stays in registers.  Meanwhile every thread takes 8 channels of one row through the convolution (the taps' rows come
+// straight from the rows and the ring), k_dim / 8 neighbours make a unit vector of them and store it as two bf16 terms in operand
+// order; the last wave makes D_ij = exp(sum of g from j, exclusive, to i) along the root paths.  From D and the products k_i.k_j,
+// q_i.k_j the first two waves make the 16 x 16 matrices
+//     T = (I + A)^-1,  A_ij = beta_i D_ij k_i.k_j (j a strict ancestor of i),    P_ij = D_ij q_i.k_j (j an ancestor or i)
+// while the others go on to KS = k S, QS = q S (three bf16 products each: 2^-17, see split2).  Then, for all rows at once,
+// u = T beta (v - e^G KS), o = e^G QS + P u, and for final rows S <- e^G_end S + sum_i D_end,i k_i u_i (f32 matrix instructions).
+// With many sequences the state's bytes bound it, with one the chain of loads and three barriers.
 // Operand order of the contraction over k_dim: lane group gq of the 16x16x32 instruction takes elements 4 gq .. + 3 of both
 // 16-wide halves of its 32, so that two neighbouring D tiles of the f32 update are exactly one B operand.
 
@@ -144,15 +145,24 @@ struct StepArgs {
     uint16_t* out;
     int64_t out_stride;
     int32_t total_rows, max_rows;
+    uint32_t inv_pv;
 };
 
+template <int DK>
+constexpr int step_lds = 16 * (DK / 32 * 64) + 256 + 3 * 320 + 2 * 16;  // floats beside k, v and the sums of squares
+
 template <int DK, bool F16, int THREADS>
-__global__ __launch_bounds__(THREADS) void k_gdn_step(GdnShape sh, GdnBatch bt, StepArgs p) {
-    extern __shared__ uint4 step_lds[];
-    const int h = blockIdx.x, s = blockIdx.y, hk = h / sh.rep, dv = sh.dv, nt = blockDim.x, tid = threadIdx.x;
-    const int lane = tid & 63, wave = tid >> 6, l16 = lane & 15, gq = lane >> 4;
+__global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step(GdnShape sh, StepArgs p, GdnBatch bt) {
+    extern __shared__ uint4 lds4[];
+    // all arguments asked for together: each trip to them takes about 0.2 us
+    asm volatile("" ::"s"(sh.hk), "s"(sh.hv), "s"(sh.rep), "s"(sh.dv), "s"(sh.taps), "s"(sh.channels), "s"(sh.conv), "s"(sh.a_log), "s"(sh.dt_bias), "s"(sh.norm));
+    asm volatile("" ::"s"(p.qkv), "s"(p.qkv_stride), "s"(p.a), "s"(p.b), "s"(p.gate_stride), "s"(p.z), "s"(p.z_stride), "s"(p.ring), "s"(p.state_in), "s"(p.state_out),
+                 "s"(p.record), "s"(p.out), "s"(p.out_stride), "s"(p.total_rows), "s"(p.max_rows), "s"(p.inv_pv), "s"(bt.base), "s"(bt.parent));
+    const int hk = blockIdx.y, h = hk * sh.rep + blockIdx.x, s = blockIdx.z, dv = sh.dv, nt = dv * 4, tid = threadIdx.x;
     const int first = bt.off[s], m = bt.off[s + 1] - first, taps = sh.taps;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, gq = lane >> 4, waves = dv >> 4;
     const int64_t base = bt.base[s];
+    const float a_log = sh.a_log[h], dt_bias = sh.dt_bias[h];
     const size_t at = ((size_t)s * sh.hv + h) * dv * DK + (size_t)(16 * wave + l16) * DK + 4 * gq;
     constexpr int NT = DK / 16;
     float4 S[NT];
@@ -165,247 +175,286 @@ __global__ __launch_bounds__(THREADS) void k_gdn_step(GdnShape sh, GdnBatch bt, 
         }
         return;
     }
-    // LDS: the convolved rows, the operand fragments (or, before them, the raw rows), the small matrices
-    const int cn = 2 * DK + dv, mr = p.max_rows;
-    float* ys = (float*)step_lds;                          // [row][q | k | v]
-    float* xs = ys + mr * cn;                              // [taps - 1 + row][..], dead once convolved
-    uint4* kf = (uint4*)xs;                                // [q, k][hi, lo][DK / 32][lane]
+    const int col = 16 * wave + l16;  // this lane's value channel; its rows are 4 gq .. + 3
+    uint16_t zr[4];
+    float nw = 0.0f;
+    if (p.z) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) zr[r] = p.z[(int64_t)(first + min(4 * gq + r, m - 1)) * p.z_stride + h * dv + col];
+        nw = sh.norm[col];
+    }
     constexpr int FR = DK / 32 * 64;
-    const int big = max((taps - 1 + mr) * cn, 16 * FR);
-    float* D = xs + big;                                   // [16][16], zero where j is no ancestor of i
-    float* A = D + 256;                                    // [16][20]
+    uint4* kf = lds4;                 // operand fragments [q, k][hi, lo][DK / 32][lane]
+    float* D = (float*)(kf + 4 * FR);  // [16][16], zero where j is no ancestor of i
+    float* A = D + 256;               // [16][20]
     float* T = A + 320;
     float* P = T + 320;
     float* beta = P + 320;
     float* eG = beta + 16;
-    float* gs = eG + 16;
-    float* red = gs + 16;                                  // [wave][16]
-    int* par = (int*)(red + 16 * (nt >> 6));
-    int* anc = par + 16;                                   // [16][4]: the row j steps back, as a row of xs
-    if (tid < 16) {
-        const int i = tid;
+    float* kv = eG + 16;              // k as f32 [m][DK], v [m][dv]
+    float* vv = kv + p.max_rows * DK;
+    float* red = vv + p.max_rows * dv;  // [row][16]: a wave's sum of squares each
+    // every wave knows the rows' parents, each sixteen lanes again
+    int par = l16 - 1;
+    if (bt.parent) {
+        par = l16 < m ? bt.parent[first + l16] : -1;
+        if (par >= l16) par = -1;
+    }
+    if (par < 0) par = -1;
+    if (wave == waves - 1) {
         float g = 0.0f, be = 0.0f;
-        int pr = i - 1;
-        if (i < m) {
-            const int64_t row = first + i;
-            g = decay_of(sh.a_log[h], row_f32<F16>(p.a[row * p.gate_stride + h]) + sh.dt_bias[h]);
+        if (l16 < m) {
+            const int64_t row = first + l16;
+            g = decay_of(a_log, row_f32<F16>(p.a[row * p.gate_stride + h]) + dt_bias);
             be = sigmoid_f32(row_f32<F16>(p.b[row * p.gate_stride + h]));
-            if (bt.parent) {
-                pr = bt.parent[row];
-                if (pr < 0 || pr >= i) pr = -1;
-            }
-            if (p.record) p.record[(size_t)p.total_rows * (sh.hv * dv + sh.hk * DK) + (size_t)row * sh.hv + h] = g;
+            if (p.record && gq == 0) p.record[(size_t)p.total_rows * (sh.hv * dv + sh.hk * DK) + (size_t)row * sh.hv + h] = g;
         }
-        gs[i] = g;
-        beta[i] = be;
-        par[i] = pr;
-    }
-    // the raw rows of this head's channels, history first; they go to their ring slots on the way
-    const int pieces = cn >> 3;
-    uint16_t* ring = p.ring + (int64_t)s * TSV_GDN_RING * sh.channels;
-    for (int i = tid; i < (taps - 1 + m) * pieces; i += nt) {
-        const int r = i / pieces, c = (i - r * pieces) * 8;
-        const int ch = c < DK ? hk * DK + c : c < 2 * DK ? (sh.hk + hk) * DK + c - DK : 2 * sh.hk * DK + h * dv + c - 2 * DK;
-        const int back = r - (taps - 1);
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (back >= 0) {
-            u = *(const uint4*)(p.qkv + (int64_t)(first + back) * p.qkv_stride + ch);
-            if (c >= 2 * DK || h == hk * sh.rep) *(uint4*)(ring + ((base + back) & (TSV_GDN_RING - 1)) * sh.channels + ch) = u;
-        } else if (base + back >= 0) {
-            u = *(const uint4*)(ring + ((base + back) & (TSV_GDN_RING - 1)) * sh.channels + ch);
-        }
-        row8_f32<F16>(u, xs + r * cn + c);
-    }
-    __syncthreads();
-    if (tid < 16) {
-        const int i = tid;
-        int q = i;
-        float sum = 0.0f;
-        for (int j = 0; j < 16; j++) D[i * 16 + j] = 0.0f;
-        for (int at_row = i; at_row >= 0; at_row = par[at_row]) {  // parents come before their children: at most 16 steps
-            D[i * 16 + at_row] = expf(sum);
-            sum += gs[at_row];
-        }
-        eG[i] = expf(sum);
-        for (int j = 0; j < 4; j++) {
-            anc[i * 4 + j] = max(q + taps - 1, 0);
-            q = q >= 0 ? par[q] : q - 1;
-        }
-    }
-    __syncthreads();
-    for (int c = tid; c < cn; c += nt) {
-        const int ch = c < DK ? hk * DK + c : c < 2 * DK ? (sh.hk + hk) * DK + c - DK : 2 * sh.hk * DK + h * dv + c - 2 * DK;
-        float w[4];
+        // the rows on row l16's root path, as bits: in each round the path doubles
+        uint32_t on = 1u << l16;
+        int up = par;
+        if (!bt.parent) {
+            on = (2u << l16) - 1;
+        } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++) w[j] = j < taps ? sh.conv[(int64_t)ch * taps + taps - 1 - j] : 0.0f;
-        for (int i = 0; i < m; i++) {
-            float v = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (j < taps) v = fmaf(xs[anc[i * 4 + j] * cn + c], w[j], v);
-            ys[i * cn + c] = silu_f32(v);
-        }
-    }
-    __syncthreads();
-    // unit vectors, as f32 (k, for the update and the record) and as operand fragments
-    for (int i = tid; i < 4 * DK; i += nt) {
-        const int mat = i / (2 * DK), row = (i / (DK / 8)) & 15, c8 = i & (DK / 8 - 1);
-        float x[8], sum = 0.0f;
-        float* src = ys + row * cn + mat * DK + 8 * c8;
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = row < m ? src[e] : 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) sum = fmaf(x[e], x[e], sum);
-#pragma unroll
-        for (int d = 1; d < DK / 8; d <<= 1) sum += __shfl_xor(sum, d);
-        const float f = row < m ? rsqrtf(sum + sh.l2_eps) : 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] *= f;
-        if (mat == 1 && row < m) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) src[e] = x[e];
-            if (p.record && h == hk * sh.rep) {
-                float* to = p.record + (size_t)p.total_rows * sh.hv * dv + ((size_t)(first + row) * sh.hk + hk) * DK + 8 * c8;
-#pragma unroll
-                for (int e = 0; e < 8; e++) to[e] = x[e];
-            }
-        }
-        const int step = c8 >> 2;
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int o = 8 * (c8 & 3) + 4 * e, to = (step * 64 + ((o & 15) >> 2) * 16 + row) * 2 + (o >> 4);
-            __bf16 hi[4], lo[4];
-#pragma unroll
-            for (int y = 0; y < 4; y++) split2(x[4 * e + y], hi[y], lo[y]);
-            uint2* f2 = (uint2*)(kf + mat * 2 * FR);
-            f2[to] = *(uint2*)hi;
-            f2[2 * FR + to] = *(uint2*)lo;
-        }
-    }
-    __syncthreads();
-    const uint4 *qh = kf, *ql = kf + FR, *kh = kf + 2 * FR, *kl = kf + 3 * FR;
-    const int waves = nt >> 6;
-    if (wave == 0 || wave == 1 || waves == 1) {
-        for (int which = wave; which < 2; which += waves) {  // 0: k.k -> A, T;  1: q.k -> P
-            gf4 acc = {0, 0, 0, 0};
-#pragma unroll
-            for (int t = 0; t < DK / 32; t++) {
-                const bf16x8 bh = __builtin_bit_cast(bf16x8, kh[t * 64 + lane]), bl = __builtin_bit_cast(bf16x8, kl[t * 64 + lane]);
-                const bf16x8 ah = __builtin_bit_cast(bf16x8, (which ? qh : kh)[t * 64 + lane]);
-                const bf16x8 al = __builtin_bit_cast(bf16x8, (which ? ql : kl)[t * 64 + lane]);
-                acc = mfma_bf16(ah, bh, acc);
-                acc = mfma_bf16(ah, bl, acc);
-                acc = mfma_bf16(al, bh, acc);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                const int i = 4 * gq + r;
-                const float d = D[i * 16 + l16] * acc[r];
-                if (which) P[i * 20 + l16] = d;
-                else A[i * 20 + l16] = i == l16 ? 0.0f : beta[i] * d;
-            }
-            if (which == 0) {
-                wave_lds_fence();
-                float x[16];  // column l16 of T, row after row
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float v = i == l16 ? 1.0f : 0.0f;
-                    if (i < m) {
-#pragma unroll
-                        for (int j = 0; j < i; j++) v = fmaf(-A[i * 20 + j], x[j], v);
-                    }
-                    x[i] = v;
-                    if (gq == 0) T[i * 20 + l16] = v;
+            for (int i = 0; i < 4; i++) {
+                const uint32_t more = __shfl(on, up & 15, 16);
+                const int next = __shfl(up, up & 15, 16);
+                if (up >= 0) {
+                    on |= more;
+                    up = next;
                 }
             }
         }
+        float sum[4] = {}, all = 0.0f;  // of g over the rows behind ancestor 4 gq + r, and over the whole path
+        uint32_t path[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) path[r] = on & ~__shfl(on, 4 * gq + r, 16);
+#pragma unroll 1
+        for (int t = 0; t < m; t++) {  // (not unrolled: code that runs once is paid by its length)
+            const float gt = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(g), t));
+            const uint32_t bit = 1u << t;
+            all += on & bit ? gt : 0.0f;
+#pragma unroll
+            for (int r = 0; r < 4; r++) sum[r] += path[r] & bit ? gt : 0.0f;
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) D[l16 * 16 + 4 * gq + r] = on >> (4 * gq + r) & 1 ? __expf(sum[r]) : 0.0f;
+        if (gq == 0) {
+            beta[l16] = be;
+            eG[l16] = __expf(all);
+        }
     }
+    // the convolution: items of 8 channels of a row, all rows' q, then k, then v
+    constexpr int pk = DK / 8;
+    const int pv = dv >> 3, items = m * (2 * pk + pv);
+    const uint32_t inv_pv = p.inv_pv;  // 65536 / pv, up: exact for the up to 512 items of v
+    uint16_t* ring = p.ring + (int64_t)s * TSV_GDN_RING * sh.channels;
+    for (int i0 = 64 * wave; i0 < items; i0 += nt) {
+        const int i = min(i0 + lane, items - 1);  // (lanes behind the last item do it again: the parents are read across lanes)
+        const int kind = i < m * pk ? 0 : i < 2 * m * pk ? 1 : 2, left = i - min(kind, 2) * m * pk;
+        const int row = kind < 2 ? left / pk : (int)(((uint32_t)left * inv_pv) >> 16), c = (left - row * (kind < 2 ? pk : pv)) * 8;
+        const int ch = kind == 0 ? hk * DK + c : kind == 1 ? (sh.hk + hk) * DK + c : 2 * sh.hk * DK + h * dv + c;
+        uf4 w[8];  // (w[..][3 - j]: j rows back)
+        if (taps == 4) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) w[e] = *(const uf4*)(sh.conv + (int64_t)(ch + e) * 4);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                w[e] = uf4{0, 0, 0, 0};
+                const float* from = sh.conv + (int64_t)(ch + e) * taps + taps;
+                w[e][3] = from[-1];
+                if (taps > 1) w[e][2] = from[-2];
+                if (taps > 2) w[e][1] = from[-3];
+            }
+        }
+        uint4 raw[4];
+        int q = row;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const uint16_t* from = q >= 0 ? p.qkv + (int64_t)(first + q) * p.qkv_stride : ring + ((base + q) & (TSV_GDN_RING - 1)) * sh.channels;
+            raw[j] = *(const uint4*)(from + ch);  // (every slot can be read; those of no position do not count)
+            if (j >= taps || base + q < 0) raw[j] = make_uint4(0, 0, 0, 0);
+            const int next = bt.parent ? __shfl(par, q & 15, 16) : q - 1;
+            q = q >= 0 ? next : q - 1;
+        }
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            float x[8];
+            row8_f32<F16>(raw[j], x);
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = fmaf(x[e], w[e][3 - j], y[e]);
+        }
+        if (kind == 2 || blockIdx.x == 0) *(uint4*)(ring + ((base + row) & (TSV_GDN_RING - 1)) * sh.channels + ch) = raw[0];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = silu_f32(y[e]);
+        if (kind == 2) {
+            *(float4*)(vv + row * dv + c) = make_float4(y[0], y[1], y[2], y[3]);
+            *(float4*)(vv + row * dv + c + 4) = make_float4(y[4], y[5], y[6], y[7]);
+        } else {
+            float sum = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) sum = fmaf(y[e], y[e], sum);
+            const float f = rsqrtf(sum_lanes<DK / 8>(sum) + sh.l2_eps);
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] *= f;
+            if (kind == 1) {
+                *(float4*)(kv + row * DK + c) = make_float4(y[0], y[1], y[2], y[3]);
+                *(float4*)(kv + row * DK + c + 4) = make_float4(y[4], y[5], y[6], y[7]);
+                if (p.record && blockIdx.x == 0) {
+                    float* to = p.record + (size_t)p.total_rows * sh.hv * dv + ((size_t)(first + row) * sh.hk + hk) * DK + c;
+                    *(uf4*)to = uf4{y[0], y[1], y[2], y[3]};
+                    *(uf4*)(to + 4) = uf4{y[4], y[5], y[6], y[7]};
+                }
+            }
+            uint2* f2 = (uint2*)(kf + kind * 2 * FR);
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const int o = (c & 31) + 4 * e, to = ((c >> 5) * 64 + ((o & 15) >> 2) * 16 + row) * 2 + (o >> 4);
+                uint2 hi, lo;
+                split2(y[4 * e], y[4 * e + 1], hi.x, lo.x);
+                split2(y[4 * e + 2], y[4 * e + 3], hi.y, lo.y);
+                f2[to] = hi;
+                f2[2 * FR + to] = lo;
+            }
+        }
+    }
+    for (int i = tid; i < 256; i += nt)  // waves and rows there are not
+        if ((i & 15) >= waves) red[i] = 0.0f;
+    for (int i = tid; i < 4 * FR; i += nt)
+        if ((i & 15) >= m) kf[i] = make_uint4(0, 0, 0, 0);
     __syncthreads();
+    const uint4 *qh = kf, *ql = kf + FR, *kh = kf + 2 * FR, *kl = kf + 3 * FR;
+    for (int which = wave; which < 2; which += waves) {  // 0: k.k -> A, T;  1: q.k -> P
+        gf4 acc = {0, 0, 0, 0}, acc2 = {0, 0, 0, 0};
+#pragma unroll
+        for (int t = 0; t < DK / 32; t++) {
+            const bf16x8 bh = __builtin_bit_cast(bf16x8, kh[t * 64 + lane]), bl = __builtin_bit_cast(bf16x8, kl[t * 64 + lane]);
+            const bf16x8 ah = __builtin_bit_cast(bf16x8, (which ? qh : kh)[t * 64 + lane]);
+            const bf16x8 al = __builtin_bit_cast(bf16x8, (which ? ql : kl)[t * 64 + lane]);
+            acc = mfma_bf16(ah, bh, acc);
+            acc2 = mfma_bf16(ah, bl, acc2);
+            acc2 = mfma_bf16(al, bh, acc2);
+        }
+        acc += acc2;
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const int i = 4 * gq + r;
+            const float d = D[i * 16 + l16];
+            if (which) P[i * 20 + l16] = d * acc[r];
+            else A[i * 20 + l16] = i == l16 ? 0.0f : beta[i] * d * acc[r];
+        }
+        if (which == 0) {
+            wave_lds_fence();
+            float x[16];  // column l16 of T, row after row
+#pragma unroll
+            for (int i = 0; i < 16; i++) x[i] = i == l16 ? 1.0f : 0.0f;
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                if (4 * b >= m) break;
+#pragma unroll
+                for (int i = 4 * b; i < 4 * b + 4; i++) {
+                    float a[16];
+#pragma unroll
+                    for (int j = 0; j < i; j += 4) *(float4*)(a + j) = *(const float4*)(A + i * 20 + j);
+#pragma unroll
+                    for (int j = 0; j < i; j++) x[i] = fmaf(-a[j], x[j], x[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) T[(4 * i + gq) * 20 + l16] = gq == 0 ? x[4 * i] : gq == 1 ? x[4 * i + 1] : gq == 2 ? x[4 * i + 2] : x[4 * i + 3];
+        }
+    }
     if (base == 0) {
 #pragma unroll
         for (int t = 0; t < NT; t++) S[t] = make_float4(0, 0, 0, 0);
     }
-    gf4 ks = {0, 0, 0, 0}, qs = {0, 0, 0, 0};
+    gf4 ks = {0, 0, 0, 0}, qs = {0, 0, 0, 0}, ks2 = {0, 0, 0, 0}, qs2 = {0, 0, 0, 0};
 #pragma unroll
     for (int t = 0; t < DK / 32; t++) {
-        bf16x8 sh8, sl8;
-        const float sv[8] = {S[2 * t].x, S[2 * t].y, S[2 * t].z, S[2 * t].w, S[2 * t + 1].x, S[2 * t + 1].y, S[2 * t + 1].z, S[2 * t + 1].w};
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            __bf16 hi, lo;
-            split2(sv[e], hi, lo);
-            sh8[e] = hi;
-            sl8[e] = lo;
-        }
+        uint4 sh8, sl8;
+        split2(S[2 * t].x, S[2 * t].y, sh8.x, sl8.x);
+        split2(S[2 * t].z, S[2 * t].w, sh8.y, sl8.y);
+        split2(S[2 * t + 1].x, S[2 * t + 1].y, sh8.z, sl8.z);
+        split2(S[2 * t + 1].z, S[2 * t + 1].w, sh8.w, sl8.w);
+        const bf16x8 s0 = __builtin_bit_cast(bf16x8, sh8), s1 = __builtin_bit_cast(bf16x8, sl8);
         const bf16x8 k0 = __builtin_bit_cast(bf16x8, kh[t * 64 + lane]), k1 = __builtin_bit_cast(bf16x8, kl[t * 64 + lane]);
         const bf16x8 q0 = __builtin_bit_cast(bf16x8, qh[t * 64 + lane]), q1 = __builtin_bit_cast(bf16x8, ql[t * 64 + lane]);
-        ks = mfma_bf16(k0, sh8, ks);
-        qs = mfma_bf16(q0, sh8, qs);
-        ks = mfma_bf16(k0, sl8, ks);
-        qs = mfma_bf16(q0, sl8, qs);
-        ks = mfma_bf16(k1, sh8, ks);
-        qs = mfma_bf16(q1, sh8, qs);
+        ks = mfma_bf16(k0, s0, ks);
+        qs = mfma_bf16(q0, s0, qs);
+        ks2 = mfma_bf16(k0, s1, ks2);
+        qs2 = mfma_bf16(q0, s1, qs2);
+        ks2 = mfma_bf16(k1, s0, ks2);
+        qs2 = mfma_bf16(q1, s0, qs2);
     }
-    const int col = 16 * wave + l16;  // this lane's value channel; its rows are 4 gq .. + 3
-    gf4 u = {0, 0, 0, 0}, o = {0, 0, 0, 0};
-    const float4 t4 = *(const float4*)(T + l16 * 20 + 4 * gq), p4 = *(const float4*)(P + l16 * 20 + 4 * gq);
-    const float tt[4] = {t4.x, t4.y, t4.z, t4.w}, pp[4] = {p4.x, p4.y, p4.z, p4.w};
+    float r4[4];
+    gf4 u = {0, 0, 0, 0}, o;
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         const int i = 4 * gq + r;
-        const float v = i < m ? ys[i * cn + 2 * DK + col] : 0.0f;
-        u = mfma_f32(tt[r], beta[i] * fmaf(-eG[i], ks[r], v), u);
-        o[r] = eG[i] * qs[r];
+        const float v = vv[min(i, m - 1) * dv + col], e = eG[i];  // (beta is 0 in rows there are not)
+        r4[r] = beta[i] * fmaf(-e, ks[r] + ks2[r], v);
+        o[r] = e * (qs[r] + qs2[r]);
     }
+    __syncthreads();
+    const float4 t4 = *(const float4*)(T + l16 * 20 + 4 * gq), p4 = *(const float4*)(P + l16 * 20 + 4 * gq);
+    const float tt[4] = {t4.x, t4.y, t4.z, t4.w}, pp[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+    for (int r = 0; r < 4; r++) u = mfma_f32(tt[r], r4[r], u);
 #pragma unroll
     for (int r = 0; r < 4; r++) o = mfma_f32(pp[r], u[r], o);
+    o *= sh.scale;
+    if (p.z) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const float q = sum_lanes<16>(o[r] * o[r]);
+            if (l16 == 0) red[(4 * gq + r) * 16 + wave] = q;
+        }
+    }
     if (p.record) {
 #pragma unroll
         for (int r = 0; r < 4; r++)
             if (4 * gq + r < m) p.record[((size_t)(first + 4 * gq + r) * sh.hv + h) * dv + col] = u[r];
     }
-    if (p.state_out) {
-        const float end = eG[m - 1];
-        float uw[4];
-#pragma unroll
-        for (int r = 0; r < 4; r++) uw[r] = u[r] * D[(m - 1) * 16 + 4 * gq + r];
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-            gf4 acc = {S[t].x * end, S[t].y * end, S[t].z * end, S[t].w * end};
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (r < m) {  // (rows 4, 8 and 12 ride in the same instruction as row 0)
-                    const int i = 4 * gq + r;
-                    acc = mfma_f32(i < m ? ys[i * cn + DK + 16 * t + l16] : 0.0f, uw[r], acc);
-                }
-            *(float4*)(p.state_out + at + 16 * t) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < 4; r++) o[r] *= sh.scale;
     if (p.z) {
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-            float q = o[r] * o[r];
-            for (int d = 1; d < 16; d <<= 1) q += __shfl_xor(q, d);
-            if (l16 == 0) red[wave * 16 + 4 * gq + r] = q;
-        }
         __syncthreads();
-        const float nw = sh.norm[col];
 #pragma unroll
         for (int r = 0; r < 4; r++) {
-            const int i = 4 * gq + r;
             float sum = 0.0f;
-            for (int w = 0; w < waves; w++) sum += red[w * 16 + i];
-            if (i < m) {
-                const float z = row_f32<F16>(p.z[(int64_t)(first + i) * p.z_stride + h * dv + col]);
-                o[r] *= rsqrtf(sum / (float)dv + sh.norm_eps) * nw * silu_f32(z);
+#pragma unroll
+            for (int w = 0; w < THREADS / 256; w++) {
+                const float4 t = *(const float4*)(red + (4 * gq + r) * 16 + 4 * w);
+                sum += (t.x + t.y) + (t.z + t.w);
             }
+            o[r] *= rsqrtf(sum / (float)dv + sh.norm_eps) * nw * silu_f32(row_f32<F16>(zr[r]));
         }
     }
 #pragma unroll
     for (int r = 0; r < 4; r++)
         if (4 * gq + r < m) p.out[(int64_t)(first + 4 * gq + r) * p.out_stride + h * dv + col] = row_bits<F16>(o[r]);
+    // (last: the stores of a whole head hold a compute unit's write path for a while)
+    if (p.state_out) {
+        const float end = eG[m - 1];
+#pragma unroll
+        for (int t = 0; t < NT; t++) S[t] = make_float4(S[t].x * end, S[t].y * end, S[t].z * end, S[t].w * end);
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            if (r >= m) break;  // (rows 4, 8 and 12 ride in the same instructions as row 0)
+            const int i = 4 * gq + r;
+            const float uw = u[r] * D[(m - 1) * 16 + i];  // (u is 0 in rows there are not)
+            const float* k = kv + min(i, m - 1) * DK + l16;
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const gf4 acc = mfma_f32(k[16 * t], uw, gf4{S[t].x, S[t].y, S[t].z, S[t].w});
+                S[t] = make_float4(acc[0], acc[1], acc[2], acc[3]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; t++) *(float4*)(p.state_out + at + 16 * t) = S[t];
+    }
 }
 
 // ---- accepted rows into the state -----------------------------------------------------------------------------------------------
@@ -593,13 +642,12 @@ int launch_conv(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const Co
 
 template <int DK, bool F16, int THREADS>
 int launch_step(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const StepArgs& p) {
-    const int waves = sh.dv / 16, cn = 2 * DK + sh.dv;
-    const int raw = (sh.taps - 1 + p.max_rows) * cn, frags = 16 * (DK / 32 * 64);
-    const size_t lds = sizeof(float) * (size_t)(p.max_rows * cn + (raw > frags ? raw : frags) + 256 + 3 * 320 + 3 * 16 + 16 * waves + 16 + 64);
+    const int waves = sh.dv / 16;
+    const size_t lds = sizeof(float) * (size_t)(step_lds<DK> + p.max_rows * (DK + sh.dv) + 256);
     static OncePerDevice once;
     const int rc = allow_lds((const void*)k_gdn_step<DK, F16, THREADS>, lds, once);
     if (rc) return rc;
-    hipLaunchKernelGGL((k_gdn_step<DK, F16, THREADS>), dim3(sh.hv, bt.n_seq), dim3(64 * waves), lds, st, sh, bt, p);
+    hipLaunchKernelGGL((k_gdn_step<DK, F16, THREADS>), dim3(sh.rep, sh.hk, bt.n_seq), dim3(64 * waves), lds, st, sh, p, bt);
     TSV_HIP(hipGetLastError());
     return TSV_OK;
 }
@@ -696,6 +744,7 @@ extern "C" int32_t tsv_gdn_step(void* stream, const tsv_gdn_layer* layer, const 
     p.out_stride = io->out_stride;
     p.total_rows = bt.off[bt.n_seq];
     p.max_rows = 1;
+    p.inv_pv = (65536 + sh.dv / 8 - 1) / (sh.dv / 8);
     for (int s = 0; s < bt.n_seq; s++) p.max_rows = std::max(p.max_rows, bt.off[s + 1] - bt.off[s]);
     const hipStream_t st = (hipStream_t)stream;
     const bool f16 = layer->dtype == TSV_F16, wide = sh.dv > 128;
