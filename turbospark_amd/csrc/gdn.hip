@@ -458,9 +458,10 @@ __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step(GdnShap
 }
 
 // ---- accepted rows into the state -----------------------------------------------------------------------------------------------
-// S <- e^{g_1 + .. + g_n} S + sum_i e^{g_{i+1} + .. + g_n} k_i u_i^T over the kept path.  A thread keeps four state values of COMMIT
-// value channels and the matching k of every kept row; one pass over the state, which is what bounds it.  The last workgroups of a
-// (sequence, layer) move the ring's rows: slot i takes the row of slot path[i] >= i, in ascending order by one thread.
+// S <- e^{g_1 + .. + g_n} S + sum_i e^{g_{i+1} + .. + g_n} k_i u_i^T over the kept path.  A thread keeps four state values of
+// COMMIT_PIECES neighbouring value channels; the path, the same for a workgroup, goes through scalar registers, and from it four rows'
+// k and u at a time are under way.  One pass over the state, which is what bounds it.  The last workgroups of a (sequence, layer)
+// move the ring's rows: slot i takes the row of slot path[i] >= i, in ascending order by one thread.
 constexpr int COMMIT_THREADS = 256, COMMIT_PIECES = 4;
 
 struct CommitArgs {
@@ -473,65 +474,74 @@ struct CommitArgs {
     const float* state_in;
     float* state_out;
     int64_t state_stride;
-    int32_t total_rows, state_blocks;
+    int32_t total_rows, state_blocks, blocks;  // workgroups of all heads' state, and of a head's
 };
 
 template <int DK>
-__global__ __launch_bounds__(COMMIT_THREADS) void k_gdn_commit(GdnShape sh, GdnBatch bt, CommitArgs p) {
-    const int s = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, first = bt.off[s], m = bt.off[s + 1] - first;
-    __shared__ int said[TSV_MAX_ROWS + 2], path[TSV_MAX_ROWS], kept;
-    __shared__ float g[TSV_MAX_ROWS], w[TSV_MAX_ROWS + 1];
+__global__ __launch_bounds__(COMMIT_THREADS) void k_gdn_commit(GdnShape sh, CommitArgs p, GdnBatch bt) {
+    asm volatile("" ::"s"(sh.hk), "s"(sh.hv), "s"(sh.rep), "s"(sh.dv), "s"(sh.channels), "s"(p.results), "s"(p.record), "s"(p.record_stride), "s"(p.ring_in),
+                 "s"(p.ring_out), "s"(p.ring_stride), "s"(p.state_in), "s"(p.state_out), "s"(p.state_stride), "s"(p.total_rows), "s"(p.state_blocks), "s"(p.blocks),
+                 "s"(bt.base));
+    const int s = blockIdx.y, layer = blockIdx.z, tid = threadIdx.x, first = bt.off[s], m = min(bt.off[s + 1] - first, TSV_MAX_ROWS);
+    const auto* said = uniform_memory(p.results + s);
     const int64_t base = bt.base[s];
     constexpr int PER_ROW = DK / 4, CH = COMMIT_THREADS / PER_ROW * COMMIT_PIECES;  // value channels of a workgroup
     const bool of_ring = (int)blockIdx.x >= p.state_blocks;
-    const int blocks = (sh.dv + CH - 1) / CH, h = of_ring ? 0 : (int)blockIdx.x / blocks, c0 = ((int)blockIdx.x - h * blocks) * CH;
-    const float* rec = p.record + (int64_t)layer * p.record_stride;
+    const int h = of_ring ? 0 : (int)blockIdx.x / p.blocks, c0 = ((int)blockIdx.x - h * p.blocks) * CH + tid / PER_ROW * COMMIT_PIECES;
+    const bool in = !of_ring && c0 < sh.dv;  // (v_dim is a multiple of 16: a thread's channels are all there or none)
     const int kq = (tid % PER_ROW) * 4;
-    const size_t at = (size_t)((int64_t)layer * p.state_stride) + ((size_t)s * sh.hv + h) * sh.dv * DK + kq;
+    const size_t at = (size_t)((int64_t)layer * p.state_stride) + (((size_t)s * sh.hv + h) * sh.dv + c0) * DK + kq;
     float4 S[COMMIT_PIECES];
-    int ch[COMMIT_PIECES];
 #pragma unroll
     for (int i = 0; i < COMMIT_PIECES; i++) {
-        ch[i] = of_ring ? sh.dv : c0 + tid / PER_ROW + i * (COMMIT_THREADS / PER_ROW);
         S[i] = make_float4(0, 0, 0, 0);
-        if (ch[i] < sh.dv) S[i] = *(const float4*)(p.state_in + at + (size_t)ch[i] * DK);
+        if (in) S[i] = *(const float4*)(p.state_in + at + i * DK);
     }
-    if (tid < TSV_MAX_ROWS) {
-        said[tid] = p.results[s].path[tid];
-        g[tid] = tid < m ? rec[(size_t)p.total_rows * (sh.hv * sh.dv + sh.hk * DK) + (size_t)(first + tid) * sh.hv + h] : 0.0f;
-    } else if (tid == TSV_MAX_ROWS) {
-        said[tid] = p.results[s].path_len;
-    } else if (tid == TSV_MAX_ROWS + 1) {
-        said[tid] = p.results[s].committed;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        const int rows = min(m, TSV_MAX_ROWS), len = said[TSV_MAX_ROWS];
-        const int want = min(len, said[TSV_MAX_ROWS + 1] < rows ? said[TSV_MAX_ROWS + 1] + 1 : rows);
-        int n = 0, before = -1;
-        while (n < want && said[n] > before && said[n] < rows) path[n] = before = said[n], n++;
-        kept = n;
-        float sum = 0.0f;
-        for (int i = n - 1; i >= 0; i--) {
-            w[i] = expf(sum);
-            sum += g[path[i]];
+    // the path as far as it names rows of the sequence in ascending order
+    int path[TSV_MAX_ROWS], n = 0;
+    {
+        const int kept = said->committed < m ? said->committed + 1 : m, len = said->path_len, want = min(kept, len);
+        int before = -1;
+        bool on = true;
+#pragma unroll
+        for (int i = 0; i < TSV_MAX_ROWS; i++) {
+            const int row = said->path[i];
+            on = on && i < want && row > before && row < m;
+            path[i] = on ? row : 0;  // (behind the path: a row that there is, with no weight)
+            n += on;
+            before = row;
         }
-        w[TSV_MAX_ROWS] = expf(sum);
     }
-    __syncthreads();
-    const int n = kept;
     if (of_ring) {
         const int c = (((int)blockIdx.x - p.state_blocks) * COMMIT_THREADS + tid) * 8;
         if (c >= sh.channels) return;
         const int64_t to = (int64_t)layer * p.ring_stride + (int64_t)s * TSV_GDN_RING * sh.channels + c;
-        for (int i = 0; i < n; i++) {
+#pragma unroll
+        for (int i = 0; i < TSV_MAX_ROWS; i++) {
+            if (i >= n) break;
             if (path[i] == i && p.ring_in == p.ring_out) continue;
             *(uint4*)(p.ring_out + to + ((base + i) & (TSV_GDN_RING - 1)) * sh.channels) =
                 *(const uint4*)(p.ring_in + to + ((base + path[i]) & (TSV_GDN_RING - 1)) * sh.channels);
         }
         return;
     }
-    const float end = w[TSV_MAX_ROWS];
+    if (!in) return;
+    const float* rec = p.record + (int64_t)layer * p.record_stride;
+    const float* rec_k = rec + (size_t)p.total_rows * sh.hv * sh.dv + ((size_t)first * sh.hk + h / sh.rep) * DK + kq;
+    const float* rec_u = rec + ((size_t)first * sh.hv + h) * sh.dv + c0;
+    const auto* rec_g = uniform_memory(rec + (size_t)p.total_rows * (sh.hv * sh.dv + sh.hk * DK) + (size_t)first * sh.hv + h);
+    float w[TSV_MAX_ROWS], sum = 0.0f;
+    if (n > 0) {  // (a sequence may have no rows at all)
+#pragma unroll
+        for (int i = 0; i < TSV_MAX_ROWS; i++) w[i] = i < n ? rec_g[path[i] * sh.hv] : 0.0f;
+    }
+#pragma unroll
+    for (int i = TSV_MAX_ROWS - 1; i >= 0; i--) {
+        const float g = n > 0 ? w[i] : 0.0f;
+        w[i] = i < n ? __expf(sum) : 0.0f;
+        sum += g;
+    }
+    const float end = __expf(sum);
 #pragma unroll
     for (int i = 0; i < COMMIT_PIECES; i++) {
         if (base == 0) S[i] = make_float4(0, 0, 0, 0);  // (what the buffer holds may be no number)
@@ -540,22 +550,30 @@ __global__ __launch_bounds__(COMMIT_THREADS) void k_gdn_commit(GdnShape sh, GdnB
         S[i].z *= end;
         S[i].w *= end;
     }
-    for (int j = 0; j < n; j++) {
-        const size_t row = first + path[j];
-        const uf4 k = *(const uf4*)(rec + (size_t)p.total_rows * sh.hv * sh.dv + (row * sh.hk + h / sh.rep) * DK + kq);
-        const float wj = w[j];
 #pragma unroll
-        for (int i = 0; i < COMMIT_PIECES; i++) {
-            const float u = ch[i] < sh.dv ? wj * rec[(row * sh.hv + h) * sh.dv + ch[i]] : 0.0f;
-            S[i].x = fmaf(u, k.x, S[i].x);
-            S[i].y = fmaf(u, k.y, S[i].y);
-            S[i].z = fmaf(u, k.z, S[i].z);
-            S[i].w = fmaf(u, k.w, S[i].w);
+    for (int j = 0; j < TSV_MAX_ROWS; j += 4) {
+        if (j >= n) break;
+        uf4 k[4], u[4];
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            k[r] = *(const uf4*)(rec_k + (size_t)path[j + r] * sh.hk * DK);
+            u[r] = *(const uf4*)(rec_u + (size_t)path[j + r] * sh.hv * sh.dv);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            if (j + r >= n) break;
+#pragma unroll
+            for (int i = 0; i < COMMIT_PIECES; i++) {
+                const float x = w[j + r] * u[r][i];
+                S[i].x = fmaf(x, k[r].x, S[i].x);
+                S[i].y = fmaf(x, k[r].y, S[i].y);
+                S[i].z = fmaf(x, k[r].z, S[i].z);
+                S[i].w = fmaf(x, k[r].w, S[i].w);
+            }
         }
     }
 #pragma unroll
-    for (int i = 0; i < COMMIT_PIECES; i++)
-        if (ch[i] < sh.dv) *(float4*)(p.state_out + at + (size_t)ch[i] * DK) = S[i];
+    for (int i = 0; i < COMMIT_PIECES; i++) *(float4*)(p.state_out + at + i * DK) = S[i];
 }
 
 // ---- arguments ----------------------------------------------------------------------------------------------------------------
@@ -655,9 +673,10 @@ int launch_step(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const St
 template <int DK>
 int launch_commit(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, CommitArgs& p, int layers) {
     constexpr int CH = COMMIT_THREADS / (DK / 4) * COMMIT_PIECES;
-    p.state_blocks = sh.hv * ((sh.dv + CH - 1) / CH);
+    p.blocks = (sh.dv + CH - 1) / CH;
+    p.state_blocks = sh.hv * p.blocks;
     const int ring_blocks = (sh.channels / 8 + COMMIT_THREADS - 1) / COMMIT_THREADS;
-    hipLaunchKernelGGL((k_gdn_commit<DK>), dim3(p.state_blocks + ring_blocks, bt.n_seq, layers), dim3(COMMIT_THREADS), 0, st, sh, bt, p);
+    hipLaunchKernelGGL((k_gdn_commit<DK>), dim3(p.state_blocks + ring_blocks, bt.n_seq, layers), dim3(COMMIT_THREADS), 0, st, sh, p, bt);
     TSV_HIP(hipGetLastError());
     return TSV_OK;
 }
