@@ -148,6 +148,47 @@ struct StepArgs {
     uint32_t inv_pv;
 };
 
+// the weights of 8 channels, w[..][3 - j] that of the row j back
+__device__ __forceinline__ void step_weights(const float* conv, int ch, int taps, uf4* w) {
+    if (taps == 4) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) w[e] = *(const uf4*)(conv + (int64_t)(ch + e) * 4);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            w[e] = uf4{0, 0, 0, 0};
+            const float* from = conv + (int64_t)(ch + e) * taps + taps;
+            w[e][3] = from[-1];
+            if (taps > 1) w[e][2] = from[-2];
+            if (taps > 2) w[e][1] = from[-3];
+        }
+    }
+}
+template <bool F16>
+__device__ __forceinline__ void step_convolve(const uint4* raw, const uf4* w, float* y) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        float x[8];
+        row8_f32<F16>(raw[j], x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = fmaf(x[e], w[e][3 - j], y[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = silu_f32(y[e]);
+}
+// 8 values of a head's vector, its others in the DK / 8 lanes around, to unit length
+template <int DK>
+__device__ __forceinline__ void step_unit(float* y, float eps) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) sum = fmaf(y[e], y[e], sum);
+    const float f = rsqrtf(sum_lanes<DK / 8>(sum) + eps);
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] *= f;
+}
+
 template <int DK>
 constexpr int step_lds = 16 * (DK / 32 * 64) + 256 + 3 * 320 + 2 * 16;  // floats beside k, v and the sums of squares
 
@@ -254,20 +295,8 @@ __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step(GdnShap
         const int kind = i < m * pk ? 0 : i < 2 * m * pk ? 1 : 2, left = i - min(kind, 2) * m * pk;
         const int row = kind < 2 ? left / pk : (int)(((uint32_t)left * inv_pv) >> 16), c = (left - row * (kind < 2 ? pk : pv)) * 8;
         const int ch = kind == 0 ? hk * DK + c : kind == 1 ? (sh.hk + hk) * DK + c : 2 * sh.hk * DK + h * dv + c;
-        uf4 w[8];  // (w[..][3 - j]: j rows back)
-        if (taps == 4) {
-#pragma unroll
-            for (int e = 0; e < 8; e++) w[e] = *(const uf4*)(sh.conv + (int64_t)(ch + e) * 4);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                w[e] = uf4{0, 0, 0, 0};
-                const float* from = sh.conv + (int64_t)(ch + e) * taps + taps;
-                w[e][3] = from[-1];
-                if (taps > 1) w[e][2] = from[-2];
-                if (taps > 2) w[e][1] = from[-3];
-            }
-        }
+        uf4 w[8];
+        step_weights(sh.conv, ch, taps, w);
         uint4 raw[4];
         int q = row;
 #pragma unroll
@@ -279,28 +308,13 @@ __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step(GdnShap
             q = q >= 0 ? next : q - 1;
         }
         float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            float x[8];
-            row8_f32<F16>(raw[j], x);
-#pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = fmaf(x[e], w[e][3 - j], y[e]);
-        }
+        step_convolve<F16>(raw, w, y);
         if (kind == 2 || blockIdx.x == 0) *(uint4*)(ring + ((base + row) & (TSV_GDN_RING - 1)) * sh.channels + ch) = raw[0];
-#pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = silu_f32(y[e]);
         if (kind == 2) {
             *(float4*)(vv + row * dv + c) = make_float4(y[0], y[1], y[2], y[3]);
             *(float4*)(vv + row * dv + c + 4) = make_float4(y[4], y[5], y[6], y[7]);
         } else {
-            float sum = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) sum = fmaf(y[e], y[e], sum);
-            const float f = rsqrtf(sum_lanes<DK / 8>(sum) + sh.l2_eps);
-#pragma unroll
-            for (int e = 0; e < 8; e++) y[e] *= f;
+            step_unit<DK>(y, sh.l2_eps);
             if (kind == 1) {
                 *(float4*)(kv + row * DK + c) = make_float4(y[0], y[1], y[2], y[3]);
                 *(float4*)(kv + row * DK + c + 4) = make_float4(y[4], y[5], y[6], y[7]);
@@ -454,6 +468,121 @@ __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step(GdnShap
         }
 #pragma unroll
         for (int t = 0; t < NT; t++) *(float4*)(p.state_out + at + 16 * t) = S[t];
+    }
+}
+
+// The same for one row a sequence, plain decoding: u = beta (v - e^g k S), o = e^g q S + (q.k) u, S <- e^g S + k u^T need no
+// 16 x 16 matrices and no operand fragments, and the products with the state are f32 dot products of a lane's k_dim / 4 values, summed
+// over the four lanes of a channel.  Two barriers.
+template <int DK, bool F16, int THREADS>
+__global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step_one(GdnShape sh, StepArgs p, GdnBatch bt) {
+    __shared__ float4 q4[DK / 4], k4[DK / 4];
+    __shared__ float vv[256], red[16], gate[2];
+    asm volatile("" ::"s"(sh.hk), "s"(sh.hv), "s"(sh.rep), "s"(sh.dv), "s"(sh.taps), "s"(sh.channels), "s"(sh.conv), "s"(sh.a_log), "s"(sh.dt_bias), "s"(sh.norm));
+    asm volatile("" ::"s"(p.qkv), "s"(p.qkv_stride), "s"(p.a), "s"(p.b), "s"(p.gate_stride), "s"(p.z), "s"(p.z_stride), "s"(p.ring), "s"(p.state_in), "s"(p.state_out),
+                 "s"(p.record), "s"(p.out), "s"(p.out_stride), "s"(p.total_rows), "s"(bt.base));
+    const int hk = blockIdx.y, h = hk * sh.rep + blockIdx.x, s = blockIdx.z, dv = sh.dv, tid = threadIdx.x;
+    const int row = bt.off[s], m = bt.off[s + 1] - row, taps = sh.taps;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, gq = lane >> 4, waves = dv >> 4;
+    const int64_t base = bt.base[s];
+    const size_t at = ((size_t)s * sh.hv + h) * dv * DK + (size_t)(16 * wave + l16) * DK + 4 * gq;
+    constexpr int NT = DK / 16;
+    float4 S[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) S[t] = *(const float4*)(p.state_in + at + 16 * t);
+    if (m <= 0) {  // no row: the state stays
+        if (p.state_out) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) *(float4*)(p.state_out + at + 16 * t) = base == 0 ? make_float4(0, 0, 0, 0) : S[t];
+        }
+        return;
+    }
+    const int col = 16 * wave + l16;  // this lane's value channel
+    uint16_t zr = 0;
+    float nw = 0.0f;
+    if (p.z) {
+        zr = p.z[(int64_t)row * p.z_stride + h * dv + col];
+        nw = sh.norm[col];
+    }
+    if (tid == 64 * (waves - 1)) {
+        const float g = decay_of(sh.a_log[h], row_f32<F16>(p.a[row * p.gate_stride + h]) + sh.dt_bias[h]);
+        gate[0] = __expf(g);
+        gate[1] = sigmoid_f32(row_f32<F16>(p.b[row * p.gate_stride + h]));
+        if (p.record) p.record[(size_t)p.total_rows * (sh.hv * dv + sh.hk * DK) + (size_t)row * sh.hv + h] = g;
+    }
+    if (tid < 16) red[tid] = 0.0f;
+    constexpr int pk = DK / 8;
+    const int items = 2 * pk + (dv >> 3);
+    uint16_t* ring = p.ring + (int64_t)s * TSV_GDN_RING * sh.channels;
+    for (int i = tid; i < items; i += 4 * dv) {
+        const int kind = i < pk ? 0 : i < 2 * pk ? 1 : 2, c = (i - kind * pk) * 8;
+        const int ch = kind == 0 ? hk * DK + c : kind == 1 ? (sh.hk + hk) * DK + c : 2 * sh.hk * DK + h * dv + c;
+        uf4 w[8];
+        step_weights(sh.conv, ch, taps, w);
+        uint4 raw[4];
+        raw[0] = *(const uint4*)(p.qkv + (int64_t)row * p.qkv_stride + ch);
+#pragma unroll
+        for (int j = 1; j < 4; j++) {
+            raw[j] = *(const uint4*)(ring + ((base - j) & (TSV_GDN_RING - 1)) * sh.channels + ch);  // (every slot can be read; those of no position do not count)
+            if (j >= taps || base < j) raw[j] = make_uint4(0, 0, 0, 0);
+        }
+        float y[8];
+        step_convolve<F16>(raw, w, y);
+        if (kind == 2 || blockIdx.x == 0) *(uint4*)(ring + (base & (TSV_GDN_RING - 1)) * sh.channels + ch) = raw[0];
+        if (kind < 2) step_unit<DK>(y, sh.l2_eps);
+        float4* to = kind == 0 ? q4 + c / 4 : kind == 1 ? k4 + c / 4 : (float4*)vv + c / 4;
+        to[0] = make_float4(y[0], y[1], y[2], y[3]);
+        to[1] = make_float4(y[4], y[5], y[6], y[7]);
+        if (kind == 1 && p.record && blockIdx.x == 0) {
+            float* rec = p.record + (size_t)p.total_rows * sh.hv * dv + ((size_t)row * sh.hk + hk) * DK + c;
+            *(uf4*)rec = uf4{y[0], y[1], y[2], y[3]};
+            *(uf4*)(rec + 4) = uf4{y[4], y[5], y[6], y[7]};
+        }
+    }
+    __syncthreads();
+    if (base == 0) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) S[t] = make_float4(0, 0, 0, 0);
+    }
+    float ks = 0.0f, qs = 0.0f, qk = 0.0f;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+        const float4 k = k4[4 * t + gq], q = q4[4 * t + gq];
+        ks = fmaf(k.x, S[t].x, fmaf(k.y, S[t].y, fmaf(k.z, S[t].z, fmaf(k.w, S[t].w, ks))));
+        qs = fmaf(q.x, S[t].x, fmaf(q.y, S[t].y, fmaf(q.z, S[t].z, fmaf(q.w, S[t].w, qs))));
+        qk = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, qk))));
+    }
+    float2 r;
+    r = lanes_by_16(ks), ks = r.x + r.y;
+    r = lanes_by_32(ks), ks = r.x + r.y;
+    r = lanes_by_16(qs), qs = r.x + r.y;
+    r = lanes_by_32(qs), qs = r.x + r.y;
+    r = lanes_by_16(qk), qk = r.x + r.y;
+    r = lanes_by_32(qk), qk = r.x + r.y;
+    const float e = gate[0], u = gate[1] * fmaf(-e, ks, vv[col]);
+    float o = sh.scale * fmaf(qk, u, e * qs);
+    if (p.z) {
+        const float q = sum_lanes<16>(o * o);
+        if (lane == 0) red[wave] = q;
+        __syncthreads();
+        float sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; w += 4) {
+            const float4 t = *(const float4*)(red + w);
+            sum += (t.x + t.y) + (t.z + t.w);
+        }
+        o *= rsqrtf(sum / (float)dv + sh.norm_eps) * nw * silu_f32(row_f32<F16>(zr));
+    }
+    if (gq == 0) {
+        p.out[(int64_t)row * p.out_stride + h * dv + col] = row_bits<F16>(o);
+        if (p.record) p.record[((size_t)row * sh.hv + h) * dv + col] = u;
+    }
+    if (p.state_out) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const float4 k = k4[4 * t + gq];
+            *(float4*)(p.state_out + at + 16 * t) = make_float4(fmaf(u, k.x, e * S[t].x), fmaf(u, k.y, e * S[t].y), fmaf(u, k.z, e * S[t].z), fmaf(u, k.w, e * S[t].w));
+        }
     }
 }
 
@@ -661,6 +790,11 @@ int launch_conv(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const Co
 template <int DK, bool F16, int THREADS>
 int launch_step(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const StepArgs& p) {
     const int waves = sh.dv / 16;
+    if (p.max_rows == 1) {  // (a row of 128 conversations: see k_gdn_step_one)
+        hipLaunchKernelGGL((k_gdn_step_one<DK, F16, THREADS>), dim3(sh.rep, sh.hk, bt.n_seq), dim3(64 * waves), 0, st, sh, p, bt);
+        TSV_HIP(hipGetLastError());
+        return TSV_OK;
+    }
     const size_t lds = sizeof(float) * (size_t)(step_lds<DK> + p.max_rows * (DK + sh.dv) + 256);
     static OncePerDevice once;
     const int rc = allow_lds((const void*)k_gdn_step<DK, F16, THREADS>, lds, once);
