@@ -86,29 +86,36 @@ constexpr int PS = 72;  // row stride (2-byte values) of P in LDS
 template <int DK, int TR>
 constexpr int blocks_operands = KFRAGS<DK, TR> * 64 > TR * BLK * PS / 8 ? KFRAGS<DK, TR> * 64 : TR * BLK * PS / 8;
 
+// What a head's decays are in a block.  e^{G_i - G_j} of rows in different row tiles is made of three factors of at most 1: from j to its
+// tile's end, the tiles between, and from the start of i's tile to i; inside a tile it is one exponential of a 64-bit difference.
+// (Two heads' at a time, without what can be made of the others: three workgroups fit a compute unit's LDS to the byte.)
+struct BlockGates {
+    double G[BLK];
+    float beta[BLK], from_start[BLK], to_end[BLK];
+};
+constexpr int GATE_HEADS = 2;
+
 template <int DK, bool F16>
-__global__ __launch_bounds__(256) void k_gdn_blocks(GdnShape sh, GdnBatch bt, PrefillArgs p) {
+__global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt, PrefillArgs p) {
     constexpr int TR = F16 ? 2 : 1, KS = DK / 32;
     extern __shared__ uint4 lds[];
     uint4* kf = lds;                                   // [row tile][k step][term][lane]
     uint16_t* P = (uint16_t*)lds;                      // [term][64][PS], where the operands were
     float* A = (float*)(lds + blocks_operands<DK, TR>);  // [64][MS]
     float* T = A + BLK * MS;
-    double* G = (double*)(T + BLK * MS);               // [64]
-    float* be = (float*)(G + BLK);                     // [64]
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, l16 = lane & 15, gq = lane >> 4, hk = blockIdx.y;
+    BlockGates* gates = (BlockGates*)(T + BLK * MS);   // of GATE_HEADS heads
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, gq = lane >> 4, hk = blockIdx.y;
     const int blk = blockIdx.x, s = sequence_of(p.block_of, bt.n_seq, blk);
     const int r0 = (blk - p.block_of[s]) * BLK, n = min(BLK, bt.off[s + 1] - bt.off[s] - r0);
     const int64_t row0 = bt.off[s] + r0;
     const int mine = 16 * w + l16;
-    float next_g = 0.0f, next_b = 0.0f;
+    float next_g = 0.0f, next_b = 0.0f;  // of the head this wave makes the decays of
     auto ask_gates = [&](int h) {
-        if (lane < n) {
-            next_g = p.g[(row0 + lane) * sh.hv + h];
-            next_b = p.beta[(row0 + lane) * sh.hv + h];
-        }
+        const int64_t at = (row0 + min(lane, n - 1)) * sh.hv + min(h, (hk + 1) * sh.rep - 1);
+        next_g = p.g[at];
+        next_b = p.beta[at];
     };
-    ask_gates(hk * sh.rep);
+    ask_gates(hk * sh.rep + w);
     bf16x8 kr[KS][TR], qr[KS][TR];
     uint4* rows_out = p.kt + ((int64_t)blk * sh.hk + hk) * (3 * KFRAGS<DK, TR> * 64);
 #pragma unroll
@@ -159,38 +166,71 @@ __global__ __launch_bounds__(256) void k_gdn_blocks(GdnShape sh, GdnBatch bt, Pr
         }
     }
     for (int h = hk * sh.rep; h < (hk + 1) * sh.rep; h++) {
-        const float b = next_b;
-        const float g = next_g > 0.0f ? 0.0f : next_g < -1e4f ? -1e4f : next_g;  // (e^-1e4 is 0; a sum of infinities has no differences)
-        ask_gates(min(h + 1, (hk + 1) * sh.rep - 1));
-        if (w == 0) {
-            double sum = g;
+        const int turn = (h - hk * sh.rep) % GATE_HEADS;
+        if (turn == 0) {  // the next heads, one a wave
+            if (w < GATE_HEADS && h + w < (hk + 1) * sh.rep) {
+                const float b = lane < n ? next_b : 0.0f;
+                float g = next_g > 0.0f ? 0.0f : next_g < -1e4f ? -1e4f : next_g;  // (e^-1e4 is 0; a sum of infinities has no differences)
+                if (lane >= n) g = 0.0f;
+                double sum = g;
 #pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const double up = __shfl_up(sum, d);
-                if (lane >= d) sum += up;
+                for (int d = 1; d < 64; d <<= 1) {
+                    const double up = __shfl_up(sum, d);
+                    if (lane >= d) sum += up;
+                }
+                double end[4];  // at the row tiles' ends
+#pragma unroll
+                for (int t = 0; t < 4; t++) end[t] = __shfl(sum, 16 * t + 15);
+                const double before = gq == 0 ? 0.0 : gq == 1 ? end[0] : gq == 2 ? end[1] : end[2];
+                const double mine_end = gq == 0 ? end[0] : gq == 1 ? end[1] : gq == 2 ? end[2] : end[3];
+                BlockGates& o = gates[w];
+                o.G[lane] = sum;
+                o.beta[lane] = b;
+                o.from_start[lane] = __expf((float)(sum - before));
+                o.to_end[lane] = __expf((float)(mine_end - sum));
+                float* to = p.gates + ((int64_t)blk * sh.hv + h + w) * 128;
+                to[lane] = __expf((float)sum);
+                to[64 + lane] = __expf((float)(end[3] - sum));
             }
-            G[lane] = sum;
-            be[lane] = b;
-            const double end = __shfl(sum, 63);
-            float* to = p.gates + ((int64_t)blk * sh.hv + h) * 128;
-            to[lane] = __expf((float)sum);
-            to[64 + lane] = __expf((float)(end - sum));
+            ask_gates(h + GATE_HEADS + w);
+            __syncthreads();
         }
-        __syncthreads();
+        const BlockGates& gt = gates[turn];
+        {
+            const float4 be4 = *(const float4*)(gt.beta + 16 * w + 4 * gq), st4 = *(const float4*)(gt.from_start + 16 * w + 4 * gq);
+            const float be[4] = {be4.x, be4.y, be4.z, be4.w}, st[4] = {st4.x, st4.y, st4.z, st4.w};
+            auto put_p = [&](int i, int j, float x) {
+                __bf16 hi, lo;
+                split2(x, hi, lo);
+                P[i * PS + j] = __builtin_bit_cast(uint16_t, hi);
+                if constexpr (TR == 2) P[(BLK + i) * PS + j] = __builtin_bit_cast(uint16_t, lo);
+            };
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            if (c > w) continue;
-            const int j = 16 * c + l16;
-            const double gj = G[j];
+            for (int c = 0; c < 3; c++) {
+                if (c >= w) continue;
+                const int j = 16 * c + l16;
+                float x = gt.to_end[j];
+                if (w - c > 1) x *= __expf((float)(gt.G[16 * w - 1] - gt.G[16 * c + 15]));
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int i = 16 * w + 4 * gq + r;
+                    const float d = st[r] * x;
+                    A[i * MS + j] = be[r] * d * kk[c][r];
+                    put_p(i, j, d * qk[c][r]);
+                }
+            }
+            const int j = 16 * w + l16;
+            const double gj = gt.G[j];
+            gf4 kd, qd;
+#pragma unroll
+            for (int c = 0; c < 4; c++)
+                if (c == w) kd = kk[c], qd = qk[c];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 const int i = 16 * w + 4 * gq + r;
-                const float d = j <= i ? __expf((float)(G[i] - gj)) : 0.0f;
-                A[i * MS + j] = j < i ? be[i] * d * kk[c][r] : 0.0f;
-                __bf16 hi, lo;
-                split2(j <= i ? d * qk[c][r] : 0.0f, hi, lo);
-                P[i * PS + j] = __builtin_bit_cast(uint16_t, hi);
-                if constexpr (TR == 2) P[(BLK + i) * PS + j] = __builtin_bit_cast(uint16_t, lo);
+                const float d = j <= i ? __expf((float)(gt.G[i] - gj)) : 0.0f;
+                A[i * MS + j] = j < i ? be[r] * d * kd[r] : 0.0f;
+                put_p(i, j, j <= i ? d * qd[r] : 0.0f);
             }
         }
         wave_lds_fence();
@@ -247,7 +287,7 @@ __global__ __launch_bounds__(256) void k_gdn_blocks(GdnShape sh, GdnBatch bt, Pr
             uint4 th, tl;
             float x[8];
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = j0 + e <= row ? T[row * MS + j0 + e] * be[j0 + e] : 0.0f;  // above the diagonal nothing has been written
+            for (int e = 0; e < 8; e++) x[e] = j0 + e <= row ? T[row * MS + j0 + e] * gt.beta[j0 + e] : 0.0f;  // above the diagonal nothing has been written
             split2(x[0], x[1], th.x, tl.x);
             split2(x[2], x[3], th.y, tl.y);
             split2(x[4], x[5], th.z, tl.z);
@@ -680,7 +720,7 @@ int64_t blocks_of(const GdnBatch& bt) {
 template <int DK, bool F16>
 int launch_blocks(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const PrefillArgs& p, int blocks) {
     constexpr int TR = F16 ? 2 : 1;
-    const size_t lds = (size_t)blocks_operands<DK, TR> * 16 + 2 * BLK * MS * 4 + BLK * 12;
+    const size_t lds = (size_t)blocks_operands<DK, TR> * 16 + 2 * BLK * MS * 4 + GATE_HEADS * sizeof(BlockGates);
     static OncePerDevice once;
     const int rc = allow_lds((const void*)k_gdn_blocks<DK, F16>, lds, once);
     if (rc) return rc;
