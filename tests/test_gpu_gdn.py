@@ -199,6 +199,22 @@ def test_prompt_with_alike_keys_and_wild_decays(dtype, keys, decay):
     p.check()
 
 
+@pytest.mark.parametrize("hk,hv,dk,dv,dtype,lengths,base,decay", [
+    (1, 1, 64, 64, BF, [2600], [0], "usual"),
+    (1, 2, 128, 128, BF, [2049], [7], "usual"),
+    (1, 1, 128, 48, HF, [2111], [0], "usual"),
+    (1, 1, 256, 32, BF, [2200], [3], "usual"),
+    (1, 2, 64, 32, BF, [2100, 70, 0, 2500], [5, 0, 4, 0], "usual"),
+    (1, 1, 64, 32, HF, [2300], [9], "wild"),
+])
+def test_long_prompts_of_few_heads(hk, hv, dk, dv, dtype, lengths, base, decay):
+    """Prompts that are walked in segments side by side and put together."""
+    rng = np.random.default_rng(dk + dv + len(lengths))
+    p = Prompt(rng, Layer(rng, hk, hv, dk, dv, 4, dtype), lengths, base, gated=False, decay=decay)
+    p.ly.gpu.prefill(p.batch, p.io)
+    p.check()
+
+
 @pytest.mark.parametrize("size", [1e-12, 1e12])
 def test_prompt_states_of_any_size(size):
     """Values and state far outside fp16's range: the operands' terms are bf16."""

@@ -29,8 +29,10 @@ struct PrefillArgs {
     int64_t out_stride;
     uint4 *kt, *tp;  // workspace: k, q and k transposed per (block, key head); T and P fragments per (block, value head)
     float* gates;    // ... and e^G, e^{G_end - G}
+    float* ends;     // ... and per (segment, value head) what a segment does to a state: [v_dim][k_dim] from nothing, then [k_dim][k_dim]
     int32_t tiles;   // column tiles of a head in the walk
-    int32_t block_of[TSV_GDN_MAX_SEQ + 1];
+    int32_t seg_blocks;  // blocks of a segment, the last of a sequence may have fewer
+    int32_t block_of[TSV_GDN_MAX_SEQ + 1], seg_of[TSV_GDN_MAX_SEQ + 1];  // first block and first segment of every sequence
 };
 
 // fragments (1 KiB: a wave's 16 bytes a lane) of a (block, key head): k and q by row tile, k transposed by 16 of k_dim
@@ -311,6 +313,9 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
 // them a wave here), so two-byte ones are taken together.  Everything a block reads is asked for one block ahead, into the registers
 // just used: the scheduling fences keep the compiler from asking earlier, which would take copies and, with them, waits.  The column tiles of a head read the same k, q, T and P: workgroups are numbered so that they share an
 // XCD's L2.
+// Where few heads leave most of the chip idle a sequence is cut into segments.  A block takes every column of the state alike, S -> M S + c
+// with M the same for all, so a first launch (ENDS) walks all segments but the last at once, from nothing with the rows' v and from the
+// unit matrix with v = 0; the walk of segment n then begins with n products M S + c of its own 16 NT columns.
 #define GDN_FENCE __builtin_amdgcn_sched_barrier(0)
 // (the wave that brings data into the L2 pays where one workgroup has a compute unit; k_dim 256 needs its registers)
 template <int DK, int NT>
@@ -347,7 +352,7 @@ struct Walk {
     }
 };
 
-template <int DK, bool F16, int NT>
+template <int DK, bool F16, int NT, bool ENDS>
 __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape sh, GdnBatch bt, PrefillArgs p) {
     typedef Walk<DK, F16, NT> W;
     constexpr int TR = W::TR, KS = W::KS, SD = W::SD;
@@ -356,10 +361,18 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
     const W x{lds, lane, w, l16, gq};
     // a key head's workgroups, its value heads' column tiles, are 8 apart: the same XCD
     const int y = blockIdx.x >> 3, of = p.tiles * sh.rep, ks_ = y / of * 8 + (blockIdx.x & 7), tile = y % p.tiles;
-    if (ks_ >= bt.n_seq * sh.hk) return;
-    const int s = ks_ / sh.hk, hk = ks_ - s * sh.hk, h = hk * sh.rep + y % of / p.tiles, hs = s * sh.hv + h, first = bt.off[s], rows = bt.off[s + 1] - first;
-    const int blocks = p.block_of[s + 1] - p.block_of[s];
-    const int64_t b0 = p.block_of[s];
+    const int segs = p.seg_of[bt.n_seq];
+    if (ks_ >= segs * sh.hk) return;
+    const int seg_at = ks_ / sh.hk, hk = ks_ - seg_at * sh.hk, h = hk * sh.rep + y % of / p.tiles;
+    const int s = sequence_of(p.seg_of, bt.n_seq, seg_at), seg = seg_at - p.seg_of[s], hs = s * sh.hv + h;
+    const bool last = seg_at + 1 == p.seg_of[s + 1];
+    if (ENDS && last) return;
+    const int skip = seg * p.seg_blocks, first = bt.off[s] + skip * BLK;
+    const int rows = last ? bt.off[s + 1] - first : p.seg_blocks * BLK, blocks = (rows + BLK - 1) / BLK;
+    const int64_t b0 = p.block_of[s] + skip;
+    const bool unit = ENDS && tile * 16 * NT >= sh.dv;  // columns of the unit matrix, not of the rows' v
+    const float* ends = p.ends + ((int64_t)p.seg_of[s] * sh.hv + h) * (sh.dv + DK) * DK;  // of the sequence's first segment
+    const int64_t ends_step = (int64_t)sh.hv * (sh.dv + DK) * DK;
     // uniform addresses of the block asked for, and what a lane adds to them (in bytes)
     const char* tpp = (const char*)(p.tp + (b0 * sh.hv + h) * (TFRAGS * (2 + TR) * 64));
     const char* gp = (const char*)(p.gates + (b0 * sh.hv + h) * 128);
@@ -377,8 +390,10 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         constexpr int AHEAD = 4, LINES = 3 * KFRAGS<DK, TR> * 8 + TFRAGS * (2 + TR) * 8, SHARE = 3;
         const char* kreg = (const char*)(p.kt + (b0 * sh.hk + hk) * (3 * KFRAGS<DK, TR> * 64));
         const int64_t k_step = (int64_t)sh.hk * (3 * KFRAGS<DK, TR> * 1024);
-        const char* vreg = (const char*)(p.v + (int64_t)first * p.v_stride + h * sh.dv + tile * 16 * NT);
+        const char* vreg = (const char*)(p.v + (int64_t)first * p.v_stride + h * sh.dv + (unit ? 0 : tile * 16 * NT));
         uint32_t got[AHEAD][SHARE + 1] = {};
+        if constexpr (!ENDS)
+            for (int q = 0; q < 2 * seg; q++) __builtin_amdgcn_s_barrier();
         for (int b = 0; b < blocks; b += AHEAD)
 #pragma unroll
             for (int j = 0; j < AHEAD; j++) {
@@ -429,7 +444,8 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         float2 gr;
         auto ask_v = [&](int b) {  // (rows behind the sequence's last are taken from it: T is 0 there)
             b = min(b, blocks - 1);
-            vr = *(const piece*)(vp + min(b * BLK + prow, rows - 1) * p.v_stride);
+            if (unit) vr = piece{};
+            else vr = *(const piece*)(vp + min(b * BLK + prow, rows - 1) * p.v_stride);
             if (w == 0) gr = *(const float2*)(gp + b * g_step + 8 * lane);
         };
         auto put_v = [&]() {
@@ -442,16 +458,27 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         };
         if (blocks > 0) {
             ask_v(0);
-            ask_q();
-            ask_p();
+            if constexpr (!ENDS) {
+                ask_q();
+                ask_p();
+            }
             put_v();
             ask_v(1);
         }
+        if constexpr (!ENDS)
+            for (int q = 0; q < 2 * seg; q++) __syncthreads();
         for (int b = 0; b < blocks; b++) {
             const bool more = b + 1 < blocks;  // (behind the last block the same one is asked for again)
             qp += more ? q_step : 0;
             tpp += more ? tp_step : 0;
             __syncthreads();
+            if constexpr (ENDS) {  // no rows go out: v and the decays alone
+                __syncthreads();
+                __syncthreads();
+                put_v();
+                ask_v(b + 2);
+                continue;
+            }
             bf16x8 st[KS][NT][2];
 #pragma unroll
             for (int i = 0; i < KS; i++)
@@ -513,15 +540,21 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         return;
     }
     // ---- the state's waves
-    const size_t at = ((size_t)hs * sh.dv + tile * 16 * NT + l16) * DK + 16 * SD * w + 4 * gq;
+    const int64_t at = ((int64_t)hs * sh.dv + tile * 16 * NT + l16) * DK + 16 * SD * w + 4 * gq;
     const bool fresh = bt.base[s] == 0;
     gf4 S[SD][NT];
 #pragma unroll
     for (int d = 0; d < SD; d++)
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            S[d][t] = *(const gf4*)(p.state_in + at + (size_t)16 * t * DK + 16 * d);
-            if (fresh) S[d][t] = gf4{0, 0, 0, 0};
+            if constexpr (ENDS) {
+                S[d][t] = gf4{0, 0, 0, 0};
+                const int on = tile * 16 * NT - sh.dv + 16 * t + l16 - (16 * (SD * w + d) + 4 * gq);  // the row of this lane's four that is 1
+                if (unit && on >= 0 && on < 4) S[d][t] = gf4{on == 0 ? 1.0f : 0.0f, on == 1 ? 1.0f : 0.0f, on == 2 ? 1.0f : 0.0f, on == 3 ? 1.0f : 0.0f};
+            } else {
+                S[d][t] = *(const gf4*)(p.state_in + at + (int64_t)16 * t * DK + 16 * d);
+                if (fresh) S[d][t] = gf4{0, 0, 0, 0};
+            }
         }
     const char* kp = (const char*)(p.kt + (b0 * sh.hk + hk) * (3 * KFRAGS<DK, TR> * 64) + w * KS * TR * 64);
     const char* ktp = (const char*)(p.kt + ((b0 * sh.hk + hk) * 3 + 2) * (KFRAGS<DK, TR> * 64) + SD * w * 2 * TR * 64);
@@ -556,6 +589,39 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
 #pragma unroll
             for (int t = 0; t < NT; t++) x.template put<2>(W::S_AT, (SD * w + d) >> 1, t, 2 * ((SD * w + d) & 1) + (gq >> 1), S[d][t]);
     };
+    if constexpr (!ENDS)
+        for (int q = 0; q < seg; q++) {  // the segments before this one: S <- M S + c
+            const float* c = ends + q * ends_step;
+            const float* M = c + (int64_t)sh.dv * DK;
+            put_state();
+            __syncthreads();
+#pragma unroll
+            for (int d = 0; d < SD; d++) {
+                float4 m[KS][2];
+#pragma unroll
+                for (int i = 0; i < KS; i++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) m[i][e] = *(const float4*)(M + (16 * (SD * w + d) + l16) * DK + 32 * i + 8 * gq + 4 * e);
+#pragma unroll
+                for (int t = 0; t < NT; t++) S[d][t] = *(const gf4*)(c + (int64_t)(tile * 16 * NT + 16 * t + l16) * DK + 16 * (SD * w + d) + 4 * gq);
+#pragma unroll
+                for (int i = 0; i < KS; i++) {
+                    uint4 hi, lo;
+                    split2(m[i][0].x, m[i][0].y, hi.x, lo.x);
+                    split2(m[i][0].z, m[i][0].w, hi.y, lo.y);
+                    split2(m[i][1].x, m[i][1].y, hi.z, lo.z);
+                    split2(m[i][1].z, m[i][1].w, hi.w, lo.w);
+                    const bf16x8 a[2] = {__builtin_bit_cast(bf16x8, hi), __builtin_bit_cast(bf16x8, lo)};
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        bf16x8 st[2];
+                        x.template get<2>(W::S_AT, i, t, st);
+                        S[d][t] = mfma_terms<2, 2>(a, st, S[d][t]);
+                    }
+                }
+            }
+            __syncthreads();
+        }
     if (blocks > 0) {
         ask_k();
         ask_t();
@@ -662,10 +728,26 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         ask_kt();
         put_state();
     }
+    if constexpr (ENDS) {
+        float* to = p.ends + ((int64_t)seg_at * sh.hv + h) * (sh.dv + DK) * DK;
 #pragma unroll
-    for (int d = 0; d < SD; d++)
+        for (int d = 0; d < SD; d++)
 #pragma unroll
-        for (int t = 0; t < NT; t++) *(gf4*)(p.state_out + at + (size_t)16 * t * DK + 16 * d) = S[d][t];
+            for (int t = 0; t < NT; t++) {
+                const int row = 16 * (SD * w + d) + 4 * gq, col = tile * 16 * NT + 16 * t + l16;
+                if (!unit) {
+                    *(gf4*)(to + (int64_t)col * DK + row) = S[d][t];
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; r++) to[(int64_t)sh.dv * DK + (row + r) * DK + col - sh.dv] = S[d][t][r];
+                }
+            }
+    } else if (last) {
+#pragma unroll
+        for (int d = 0; d < SD; d++)
+#pragma unroll
+            for (int t = 0; t < NT; t++) *(gf4*)(p.state_out + at + (int64_t)16 * t * DK + 16 * d) = S[d][t];
+    }
 }
 #undef GDN_FENCE
 
@@ -697,24 +779,42 @@ __global__ __launch_bounds__(256) void k_gdn_norm(GdnShape sh, uint16_t* out, in
 
 namespace {
 
-struct Sizes {
-    int64_t kt, tp, gates, total;  // bytes
-};
+int64_t blocks_of(const GdnBatch& bt, int s) { return (bt.off[s + 1] - bt.off[s] + BLK - 1) / BLK; }
 
-Sizes workspace_of(const GdnShape& sh, int dk, bool f16, int64_t blocks) {
-    const int tr = f16 ? 2 : 1;
-    Sizes z;
-    z.kt = blocks * sh.hk * (3 * (dk / 8) * tr * 1024);
-    z.tp = blocks * sh.hv * (TFRAGS * (2 + tr) * 1024);
-    z.gates = blocks * sh.hv * 512;
-    z.total = z.kt + z.tp + z.gates;
-    return z;
+// How many blocks a segment has, INT32_MAX: whole sequences.  In segments a sequence's columns are walked twice and the k_dim columns of the
+// unit matrix once, so that it pays where at most a quarter of the compute units would have a workgroup: 32768 rows of 8 heads of 128
+// (64 column tiles) took 605 us whole, 360 in 4 segments, 319 in 8, 360 in 16.  Segments of fewer than 8 blocks gain nothing over
+// what putting them together takes (1.5 us each).
+int segment_blocks(const GdnShape& sh, const GdnBatch& bt) {
+    int64_t longest = 0;
+    for (int s = 0; s < bt.n_seq; s++) longest = std::max(longest, blocks_of(bt, s));
+    const int64_t tiles = (int64_t)bt.n_seq * sh.hv * (sh.dv / 16);
+    if (tiles > 64 || longest < 32) return INT32_MAX;
+    const int64_t segs = std::min<int64_t>(512 / tiles, longest / 8);
+    return (int)((longest + segs - 1) / segs);
 }
 
-int64_t blocks_of(const GdnBatch& bt) {
-    int64_t n = 0;
-    for (int s = 0; s < bt.n_seq; s++) n += (bt.off[s + 1] - bt.off[s] + BLK - 1) / BLK;
-    return n;
+struct Sizes {
+    int64_t kt, tp, gates, ends, total;  // bytes
+    int64_t blocks, segments;
+    int seg_blocks;
+};
+
+Sizes workspace_of(const GdnShape& sh, const GdnBatch& bt, int dk, bool f16) {
+    const int tr = f16 ? 2 : 1;
+    Sizes z;
+    z.blocks = z.segments = 0;
+    z.seg_blocks = segment_blocks(sh, bt);
+    for (int s = 0; s < bt.n_seq; s++) {
+        z.blocks += blocks_of(bt, s);
+        z.segments += std::max<int64_t>(1, (blocks_of(bt, s) + z.seg_blocks - 1) / z.seg_blocks);
+    }
+    z.kt = z.blocks * sh.hk * (3 * (dk / 8) * tr * 1024);
+    z.tp = z.blocks * sh.hv * (TFRAGS * (2 + tr) * 1024);
+    z.gates = z.blocks * sh.hv * 512;
+    z.ends = z.seg_blocks == INT32_MAX ? 0 : z.segments * sh.hv * (sh.dv + dk) * dk * 4;
+    z.total = z.kt + z.tp + z.gates + z.ends;
+    return z;
 }
 
 template <int DK, bool F16>
@@ -729,15 +829,15 @@ int launch_blocks(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const 
     return TSV_OK;
 }
 
-template <int DK, bool F16, int NT>
+template <int DK, bool F16, int NT, bool ENDS>
 int launch_walk(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, PrefillArgs& p) {
     const size_t lds = (size_t)Walk<DK, F16, NT>::LDS * 16;
     static OncePerDevice once;
-    const int rc = allow_lds((const void*)k_gdn_walk<DK, F16, NT>, lds, once);
+    const int rc = allow_lds((const void*)k_gdn_walk<DK, F16, NT, ENDS>, lds, once);
     if (rc) return rc;
-    p.tiles = sh.dv / (16 * NT);
-    const int heads = bt.n_seq * sh.hk;
-    hipLaunchKernelGGL((k_gdn_walk<DK, F16, NT>), dim3((heads + 7) / 8 * 8 * sh.rep * p.tiles), dim3(walk_threads<DK, NT>), lds, st, sh, bt, p);
+    p.tiles = (sh.dv + (ENDS ? DK : 0)) / (16 * NT);
+    const int heads = p.seg_of[bt.n_seq] * sh.hk;
+    hipLaunchKernelGGL((k_gdn_walk<DK, F16, NT, ENDS>), dim3((heads + 7) / 8 * 8 * sh.rep * p.tiles), dim3(walk_threads<DK, NT>), lds, st, sh, bt, p);
     TSV_HIP(hipGetLastError());
     return TSV_OK;
 }
@@ -751,9 +851,15 @@ int launch_prefill(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, Prefi
     // Two column tiles a workgroup where that still gives every compute unit one: they share what a block reads (6 sequences, 32 heads of
     // 128: 70 us against 100); else one, for the shorter way through a block (8192 rows, 32 heads: 189 us against 219).  k_dim 256 has no
     // registers for two.
+    if (p.seg_of[bt.n_seq] > bt.n_seq) {
+        int rc;
+        if constexpr (DK < 256) rc = sh.dv % 32 == 0 ? launch_walk<DK, F16, 2, true>(st, sh, bt, p) : launch_walk<DK, F16, 1, true>(st, sh, bt, p);
+        else rc = launch_walk<DK, F16, 1, true>(st, sh, bt, p);
+        if (rc) return rc;
+    }
     if constexpr (DK < 256)
-        if (sh.dv % 32 == 0 && (int64_t)bt.n_seq * sh.hv * (sh.dv / 32) >= 256) return launch_walk<DK, F16, 2>(st, sh, bt, p);
-    return launch_walk<DK, F16, 1>(st, sh, bt, p);
+        if (sh.dv % 32 == 0 && (int64_t)p.seg_of[bt.n_seq] * sh.hv * (sh.dv / 32) >= 256) return launch_walk<DK, F16, 2, false>(st, sh, bt, p);
+    return launch_walk<DK, F16, 1, false>(st, sh, bt, p);
 }
 
 }  // namespace
@@ -766,7 +872,7 @@ extern "C" int64_t tsv_gdn_prefill_workspace(const tsv_gdn_layer* layer, const t
     GdnShape sh;
     GdnBatch bt;
     if (gdn_check("gdn_prefill_workspace", nullptr, layer, batch, 0, &sh, &bt)) return -1;
-    return std::max<int64_t>(16, workspace_of(sh, layer->k_dim, layer->dtype == TSV_F16, blocks_of(bt)).total);
+    return std::max<int64_t>(16, workspace_of(sh, bt, layer->k_dim, layer->dtype == TSV_F16).total);
 }
 
 extern "C" int32_t tsv_gdn_prefill(void* stream, const tsv_gdn_layer* layer, const tsv_gdn_batch* batch, const tsv_gdn_prefill_io* io) {
@@ -786,8 +892,8 @@ extern "C" int32_t tsv_gdn_prefill(void* stream, const tsv_gdn_layer* layer, con
     if (io->out == io->q || io->out == io->k || io->out == io->v || io->out == io->z) return gdn_refuse(who, "out may not be the input rows");
     if (gdn_overlap(io->state_in, io->state_out, sizeof(float) * (size_t)(bt.n_seq * vw * dk))) return gdn_refuse(who, "state_out overlaps state_in");
     const bool f16 = layer->dtype == TSV_F16;
-    const int64_t blocks = blocks_of(bt);
-    const Sizes z = workspace_of(sh, dk, f16, blocks);
+    const Sizes z = workspace_of(sh, bt, dk, f16);
+    const int64_t blocks = z.blocks;
     if (io->workspace_bytes < z.total) return gdn_refuse(who, "the workspace is smaller than tsv_gdn_prefill_workspace says");
     PrefillArgs p;
     p.q = (const uint16_t*)io->q;
@@ -806,8 +912,13 @@ extern "C" int32_t tsv_gdn_prefill(void* stream, const tsv_gdn_layer* layer, con
     p.kt = (uint4*)ws;
     p.tp = (uint4*)(ws + z.kt);
     p.gates = (float*)(ws + z.kt + z.tp);
-    p.block_of[0] = 0;
-    for (int s = 0; s < bt.n_seq; s++) p.block_of[s + 1] = p.block_of[s] + (bt.off[s + 1] - bt.off[s] + BLK - 1) / BLK;
+    p.ends = (float*)(ws + z.kt + z.tp + z.gates);
+    p.seg_blocks = z.seg_blocks;
+    p.block_of[0] = p.seg_of[0] = 0;
+    for (int s = 0; s < bt.n_seq; s++) {
+        p.block_of[s + 1] = p.block_of[s] + (int32_t)blocks_of(bt, s);
+        p.seg_of[s + 1] = p.seg_of[s] + (int32_t)std::max<int64_t>(1, (blocks_of(bt, s) + z.seg_blocks - 1) / z.seg_blocks);
+    }
     const hipStream_t st = (hipStream_t)stream;
     int done;
     if (dk == 64) done = f16 ? launch_prefill<64, true>(st, sh, bt, p, (int)blocks) : launch_prefill<64, false>(st, sh, bt, p, (int)blocks);
