@@ -31,6 +31,7 @@ struct PrefillArgs {
     float* gates;    // ... and e^G, e^{G_end - G}
     float* ends;     // ... and per (segment, value head) what a segment does to a state: [v_dim][k_dim] from nothing, then [k_dim][k_dim]
     int32_t tiles;   // column tiles of a head in the walk
+    int32_t split;   // the blocks' matrices: a workgroup per value head
     int32_t seg_blocks;  // blocks of a segment, the last of a sequence may have fewer
     int32_t block_of[TSV_GDN_MAX_SEQ + 1], seg_of[TSV_GDN_MAX_SEQ + 1];  // first block and first segment of every sequence
 };
@@ -82,7 +83,8 @@ __device__ __forceinline__ int sequence_of(const int32_t* starts, int n, int at)
 // One workgroup per (block, key head), wave w owning rows 16 w ..; the products k.k and q.k are made once and shared by the key head's
 // value heads, whose decays make A and P of them.  The inverse: each wave inverts its 16 x 16 diagonal block row by row, a column a
 // lane; then wave j does the blocks under diagonal block j, T_ij = -T_ii sum_l A_il T_lj, on the f32 matrix instruction, whose D layout
-// is its B operand's when the contraction takes rows 4 gq + r in step r.
+// is its B operand's when the contraction takes rows 4 gq + r in step r.  Few blocks have a workgroup per value head instead (split), each
+// making the products again: 65 rows, 8 heads over 4, 14.4 us against 10.1.
 constexpr int PS = 72;  // row stride (2-byte values) of P in LDS
 // 16-byte units of LDS that hold k's operands, then P
 template <int DK, int TR>
@@ -106,18 +108,20 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
     float* A = (float*)(lds + blocks_operands<DK, TR>);  // [64][MS]
     float* T = A + BLK * MS;
     BlockGates* gates = (BlockGates*)(T + BLK * MS);   // of GATE_HEADS heads
-    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, gq = lane >> 4, hk = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, gq = lane >> 4;
+    const int hk = p.split ? blockIdx.y / sh.rep : blockIdx.y, h0 = p.split ? blockIdx.y : hk * sh.rep, h1 = p.split ? h0 + 1 : h0 + sh.rep;
+    const bool writes = h0 == hk * sh.rep;  // k, q and k transposed, for all of the key head's value heads
     const int blk = blockIdx.x, s = sequence_of(p.block_of, bt.n_seq, blk);
     const int r0 = (blk - p.block_of[s]) * BLK, n = min(BLK, bt.off[s + 1] - bt.off[s] - r0);
     const int64_t row0 = bt.off[s] + r0;
     const int mine = 16 * w + l16;
     float next_g = 0.0f, next_b = 0.0f;  // of the head this wave makes the decays of
     auto ask_gates = [&](int h) {
-        const int64_t at = (row0 + min(lane, n - 1)) * sh.hv + min(h, (hk + 1) * sh.rep - 1);
+        const int64_t at = (row0 + min(lane, n - 1)) * sh.hv + min(h, h1 - 1);
         next_g = p.g[at];
         next_b = p.beta[at];
     };
-    ask_gates(hk * sh.rep + w);
+    ask_gates(h0 + w);
     bf16x8 kr[KS][TR], qr[KS][TR];
     uint4* rows_out = p.kt + ((int64_t)blk * sh.hk + hk) * (3 * KFRAGS<DK, TR> * 64);
 #pragma unroll
@@ -133,8 +137,8 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
         for (int e = 0; e < TR; e++) {
             const int f = (w * KS + t) * TR + e;
             kf[f * 64 + lane] = __builtin_bit_cast(uint4, kr[t][e]);
-            rows_out[f * 64 + lane] = __builtin_bit_cast(uint4, kr[t][e]);
-            rows_out[(KFRAGS<DK, TR> + f) * 64 + lane] = __builtin_bit_cast(uint4, qr[t][e]);
+            if (writes) rows_out[f * 64 + lane] = __builtin_bit_cast(uint4, kr[t][e]);
+            if (writes) rows_out[(KFRAGS<DK, TR> + f) * 64 + lane] = __builtin_bit_cast(uint4, qr[t][e]);
         }
     }
     __syncthreads();
@@ -153,7 +157,7 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
         }
     }
     // k transposed, as the operand of the state's update: rows k_dim, eight block rows a lane
-    {
+    if (writes) {
         const uint16_t* kh = (const uint16_t*)kf;
         uint4* to = rows_out + 2 * KFRAGS<DK, TR> * 64;
         for (int f = w; f < DK / 16 * 2 * TR; f += 4) {
@@ -167,10 +171,10 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
             to[f * 64 + lane] = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16);
         }
     }
-    for (int h = hk * sh.rep; h < (hk + 1) * sh.rep; h++) {
-        const int turn = (h - hk * sh.rep) % GATE_HEADS;
+    for (int h = h0; h < h1; h++) {
+        const int turn = (h - h0) % GATE_HEADS;
         if (turn == 0) {  // the next heads, one a wave
-            if (w < GATE_HEADS && h + w < (hk + 1) * sh.rep) {
+            if (w < GATE_HEADS && h + w < h1) {
                 const float b = lane < n ? next_b : 0.0f;
                 float g = next_g > 0.0f ? 0.0f : next_g < -1e4f ? -1e4f : next_g;  // (e^-1e4 is 0; a sum of infinities has no differences)
                 if (lane >= n) g = 0.0f;
@@ -317,6 +321,11 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
 // with M the same for all, so a first launch (ENDS) walks all segments but the last at once, from nothing with the rows' v and from the
 // unit matrix with v = 0; the walk of segment n then begins with n products M S + c of its own 16 NT columns.
 #define GDN_FENCE __builtin_amdgcn_sched_barrier(0)
+// all loads have arrived, and the compiler knows: what is under way before a loop would else count in every wait inside it
+#define GDN_ARRIVED                            \
+    GDN_FENCE;                                 \
+    __builtin_amdgcn_s_waitcnt(0x0F70);        \
+    GDN_FENCE
 // (the wave that brings data into the L2 pays where one workgroup has a compute unit; k_dim 256 needs its registers)
 template <int DK, int NT>
 constexpr int walk_threads = NT == 1 && DK < 256 ? 576 : 512;
@@ -434,7 +443,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         // a lane's piece of the rows: a quarter of row lane / 4 of the wave's sixteen
         typedef uint32_t piece __attribute__((ext_vector_type(2 * NT)));
         const int prow = 16 * w + (lane >> 2), pcol = (lane & 3) * 4 * NT;
-        const uint16_t* vp = p.v + (int64_t)first * p.v_stride + h * sh.dv + tile * 16 * NT + pcol;
+        const uint16_t* vp = p.v + (int64_t)first * p.v_stride + h * sh.dv + (unit ? 0 : tile * 16 * NT) + pcol;
         char* op = (char*)(p.out + (int64_t)first * p.out_stride + h * sh.dv + tile * 16 * NT);
         const int64_t o_step = p.out_stride * (2 * BLK);
         const uint32_t o_off = prow * (uint32_t)(2 * p.out_stride) + 2 * pcol;
@@ -444,18 +453,20 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         float2 gr;
         auto ask_v = [&](int b) {  // (rows behind the sequence's last are taken from it: T is 0 there)
             b = min(b, blocks - 1);
-            if (unit) vr = piece{};
-            else vr = *(const piece*)(vp + min(b * BLK + prow, rows - 1) * p.v_stride);
-            if (w == 0) gr = *(const float2*)(gp + b * g_step + 8 * lane);
+            vr = *(const piece*)(vp + min(b * BLK + prow, rows - 1) * p.v_stride);
+            gr = *(const float2*)(gp + b * g_step + 8 * lane);
         };
         auto put_v = [&]() {
 #pragma unroll
             for (int i = 0; i < 2 * NT; i++) {
-                vt[(pcol + 2 * i) * W::VS + prow] = (uint16_t)vr[i];
-                vt[(pcol + 2 * i + 1) * W::VS + prow] = (uint16_t)(vr[i] >> 16);
+                const uint32_t two = ENDS && unit ? 0 : vr[i];
+                vt[(pcol + 2 * i) * W::VS + prow] = (uint16_t)two;
+                vt[(pcol + 2 * i + 1) * W::VS + prow] = (uint16_t)(two >> 16);
             }
             if (w == 0) ((float2*)(lds + W::G_AT))[lane] = gr;
         };
+        if constexpr (!ENDS)
+            for (int q = 0; q < 2 * seg; q++) __syncthreads();
         if (blocks > 0) {
             ask_v(0);
             if constexpr (!ENDS) {
@@ -464,9 +475,8 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
             }
             put_v();
             ask_v(1);
+            GDN_ARRIVED;
         }
-        if constexpr (!ENDS)
-            for (int q = 0; q < 2 * seg; q++) __syncthreads();
         for (int b = 0; b < blocks; b++) {
             const bool more = b + 1 < blocks;  // (behind the last block the same one is asked for again)
             qp += more ? q_step : 0;
@@ -475,7 +485,9 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
             if constexpr (ENDS) {  // no rows go out: v and the decays alone
                 __syncthreads();
                 __syncthreads();
+                GDN_FENCE;
                 put_v();
+                GDN_FENCE;
                 ask_v(b + 2);
                 continue;
             }
@@ -627,6 +639,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         ask_t();
         ask_kt();
         put_state();
+        GDN_ARRIVED;
     }
     for (int b = 0; b < blocks; b++) {
         const bool more = b + 1 < blocks;
@@ -750,6 +763,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
     }
 }
 #undef GDN_FENCE
+#undef GDN_ARRIVED
 
 // ---- the gated norm, in place --------------------------------------------------------------------------------------------------------
 // v_dim / 8 of GROUP neighbouring lanes hold a head's row.
@@ -818,13 +832,14 @@ Sizes workspace_of(const GdnShape& sh, const GdnBatch& bt, int dk, bool f16) {
 }
 
 template <int DK, bool F16>
-int launch_blocks(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const PrefillArgs& p, int blocks) {
+int launch_blocks(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, PrefillArgs& p, int blocks) {
     constexpr int TR = F16 ? 2 : 1;
     const size_t lds = (size_t)blocks_operands<DK, TR> * 16 + 2 * BLK * MS * 4 + GATE_HEADS * sizeof(BlockGates);
     static OncePerDevice once;
     const int rc = allow_lds((const void*)k_gdn_blocks<DK, F16>, lds, once);
     if (rc) return rc;
-    hipLaunchKernelGGL((k_gdn_blocks<DK, F16>), dim3(blocks, sh.hk), dim3(256), lds, st, sh, bt, p);
+    p.split = sh.rep > 1 && (int64_t)blocks * sh.hk < 512;
+    hipLaunchKernelGGL((k_gdn_blocks<DK, F16>), dim3(blocks, p.split ? sh.hv : sh.hk), dim3(256), lds, st, sh, bt, p);
     TSV_HIP(hipGetLastError());
     return TSV_OK;
 }
