@@ -7,9 +7,11 @@
 // sequence with 16 NT columns of one head's state in registers, k_gdn_norm is the gated norm of the result.
 //
 // Precision: the state is f32 and never rounded; as operands of the bf16 matrix instruction the state, T, u and the difference
-// v - e^G kS are two bf16 terms each (2^-18, split2), k and q the rows' own bits (fp16 rows: two terms, exact).  P u, which ends in
-// a rounding to the rows' type, is one term by one for bf16 rows and two by two for fp16.  T's inverse is f32 throughout, the running
-// sum of g 64 bits, since differences of a long sum are what the decays are made of.
+// v - e^G kS are two bf16 terms each (2^-18, split2: 5e-6 of the state's norm after thousands of rows; one term would leave 2e-3), k and
+// q the rows' own bits (fp16 rows: two terms, exact).  P u, which ends in a rounding to the rows' type, is one term by one for bf16 rows
+// (2.5e-3 of the result's norm with that rounding's 1.7e-3 in it; two by two costs the walk 15%) and two by two for fp16.  T's inverse is
+// f32 throughout, the running sum of g 64 bits, since differences of a long sum are what the decays are made of.  o is rounded to the
+// rows' type before the gated norm reads it again: half a step more in the result, where f32 would move twice the bytes.
 #include "gdn.h"
 
 #include <algorithm>
@@ -710,7 +712,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
             for (int t = 0; t < NT; t++) {
                 u[t] += u2[t];
                 x.template put<2>(W::D_AT, w >> 1, t, 2 * (w & 1) + (gq >> 1), ed * u[t]);
-                x.template put<TR>(W::U_AT, w >> 1, t, 2 * (w & 1) + (gq >> 1), u[t]);
+                if constexpr (!ENDS) x.template put<TR>(W::U_AT, w >> 1, t, 2 * (w & 1) + (gq >> 1), u[t]);
             }
 #pragma unroll
             for (int i = 0; i < SD; i++)
