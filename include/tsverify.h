@@ -468,7 +468,8 @@ int64_t tsv_vocab(const tsv_ctx* ctx);
  * from nothing, whatever its state and ring hold.
  *
  * Rows are bf16 or fp16.  Strides are elements from row to row, multiples of 8, at most 2^22; qkv, q, k, v, z, out and the rings are 16-byte
- * aligned.  Rows outside the batch's sequences are neither read nor written.  Outputs must not overlap inputs, but for state_out
+ * aligned.  Rows outside the batch's sequences are neither read nor written.  A row that holds no number spoils its own sequence: the
+ * rows behind it, and those of its block or pass.  Outputs must not overlap inputs, but for state_out
  * == state_in and ring_out == ring_in. */
 #define TSV_GDN_RING 32     /* raw rows kept per sequence: conv_width - 1 behind a pass and TSV_MAX_ROWS of it */
 #define TSV_GDN_MAX_SEQ 256 /* sequences of one call */

@@ -32,6 +32,7 @@ struct PrefillArgs {
     uint4 *kt, *tp;  // workspace: k, q and k transposed per (block, key head); T and P fragments per (block, value head)
     float* gates;    // ... and e^G, e^{G_end - G}
     float* ends;     // ... and per (segment, value head) what a segment does to a state: [v_dim][k_dim] from nothing, then [k_dim][k_dim]
+    float* starts;   // ... and the states that sequences of several segments start from: state_out may be state_in
     int32_t tiles;   // column tiles of a head in the walk
     int32_t split;   // the blocks' matrices: a workgroup per value head
     int32_t seg_blocks;  // blocks of a segment, the last of a sequence may have fewer
@@ -377,6 +378,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
     const int seg_at = ks_ / sh.hk, hk = ks_ - seg_at * sh.hk, h = hk * sh.rep + y % of / p.tiles;
     const int s = sequence_of(p.seg_of, bt.n_seq, seg_at), seg = seg_at - p.seg_of[s], hs = s * sh.hv + h;
     const bool last = seg_at + 1 == p.seg_of[s + 1];
+    const bool whole = seg == 0 && last;
     if (ENDS && last) return;
     const int skip = seg * p.seg_blocks, first = bt.off[s] + skip * BLK;
     const int rows = last ? bt.off[s + 1] - first : p.seg_blocks * BLK, blocks = (rows + BLK - 1) / BLK;
@@ -562,11 +564,13 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
 #pragma unroll
         for (int t = 0; t < NT; t++) {
             if constexpr (ENDS) {
+                // (the last segment writes state_out while others may still have to read theirs: they read a copy)
+                if (seg == 0 && !unit) *(gf4*)(p.starts + at + (int64_t)16 * t * DK + 16 * d) = *(const gf4*)(p.state_in + at + (int64_t)16 * t * DK + 16 * d);
                 S[d][t] = gf4{0, 0, 0, 0};
                 const int on = tile * 16 * NT - sh.dv + 16 * t + l16 - (16 * (SD * w + d) + 4 * gq);  // the row of this lane's four that is 1
                 if (unit && on >= 0 && on < 4) S[d][t] = gf4{on == 0 ? 1.0f : 0.0f, on == 1 ? 1.0f : 0.0f, on == 2 ? 1.0f : 0.0f, on == 3 ? 1.0f : 0.0f};
             } else {
-                S[d][t] = *(const gf4*)(p.state_in + at + (int64_t)16 * t * DK + 16 * d);
+                S[d][t] = *(const gf4*)((whole ? p.state_in : p.starts) + at + (int64_t)16 * t * DK + 16 * d);
                 if (fresh) S[d][t] = gf4{0, 0, 0, 0};
             }
         }
@@ -771,26 +775,28 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
 // v_dim / 8 of GROUP neighbouring lanes hold a head's row.
 template <bool F16>
 __global__ __launch_bounds__(256) void k_gdn_norm(GdnShape sh, uint16_t* out, int64_t out_stride, const uint16_t* z, int64_t z_stride, int64_t heads, int group) {
-    const int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / group;
-    const int c = (threadIdx.x & (group - 1)) * 8;
-    const bool in = at < heads && c < sh.dv;
-    const int64_t row = at / sh.hv;
-    const int h = (int)(at - row * sh.hv);
-    uint16_t* o = out + row * out_stride + h * sh.dv + c;
-    float x[8] = {}, y[8] = {}, sum = 0.0f;
-    if (in) {
-        row8_f32<F16>(*(const uint4*)o, x);
-        row8_f32<F16>(*(const uint4*)(z + row * z_stride + h * sh.dv + c), y);
+    const int c = (threadIdx.x & (group - 1)) * 8, a_wg = 256 / group;
+    for (int64_t first = (int64_t)blockIdx.x * a_wg; first < heads; first += (int64_t)gridDim.x * a_wg) {
+        const int64_t at = first + threadIdx.x / group;
+        const int64_t row = heads <= INT32_MAX ? (int64_t)((uint32_t)at / (uint32_t)sh.hv) : at / sh.hv;
+        const bool in = at < heads && c < sh.dv;
+        const int h = (int)(at - row * sh.hv);
+        uint16_t* o = out + row * out_stride + h * sh.dv + c;
+        float x[8] = {}, y[8] = {}, sum = 0.0f;
+        if (in) {
+            row8_f32<F16>(*(const uint4*)o, x);
+            row8_f32<F16>(*(const uint4*)(z + row * z_stride + h * sh.dv + c), y);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) sum = fmaf(x[e], x[e], sum);
+        for (int d = 1; d < group; d <<= 1) sum += __shfl_xor(sum, d);
+        if (in) {
+            const float f = rsqrtf(sum / (float)sh.dv + sh.norm_eps);
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] *= f * sh.norm[c + e] * silu_f32(y[e]);
+            *(uint4*)o = make_uint4(row_pair<F16>(x[0], x[1]), row_pair<F16>(x[2], x[3]), row_pair<F16>(x[4], x[5]), row_pair<F16>(x[6], x[7]));
+        }
     }
-#pragma unroll
-    for (int e = 0; e < 8; e++) sum = fmaf(x[e], x[e], sum);
-    for (int d = 1; d < group; d <<= 1) sum += __shfl_xor(sum, d);
-    if (!in) return;
-    const float f = rsqrtf(sum / (float)sh.dv + sh.norm_eps);
-    uint32_t b[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) b[e] = row_bits<F16>(x[e] * f * sh.norm[c + e] * silu_f32(y[e]));
-    *(uint4*)o = make_uint4(b[0] | b[1] << 16, b[2] | b[3] << 16, b[4] | b[5] << 16, b[6] | b[7] << 16);
 }
 
 namespace {
@@ -811,7 +817,7 @@ int segment_blocks(const GdnShape& sh, const GdnBatch& bt) {
 }
 
 struct Sizes {
-    int64_t kt, tp, gates, ends, total;  // bytes
+    int64_t kt, tp, gates, ends, starts, total;  // bytes
     int64_t blocks, segments;
     int seg_blocks;
 };
@@ -829,7 +835,8 @@ Sizes workspace_of(const GdnShape& sh, const GdnBatch& bt, int dk, bool f16) {
     z.tp = z.blocks * sh.hv * (TFRAGS * (2 + tr) * 1024);
     z.gates = z.blocks * sh.hv * 512;
     z.ends = z.seg_blocks == INT32_MAX ? 0 : z.segments * sh.hv * (sh.dv + dk) * dk * 4;
-    z.total = z.kt + z.tp + z.gates + z.ends;
+    z.starts = z.seg_blocks == INT32_MAX ? 0 : (int64_t)bt.n_seq * sh.hv * sh.dv * dk * 4;
+    z.total = z.kt + z.tp + z.gates + z.ends + z.starts;
     return z;
 }
 
@@ -930,6 +937,7 @@ extern "C" int32_t tsv_gdn_prefill(void* stream, const tsv_gdn_layer* layer, con
     p.tp = (uint4*)(ws + z.kt);
     p.gates = (float*)(ws + z.kt + z.tp);
     p.ends = (float*)(ws + z.kt + z.tp + z.gates);
+    p.starts = (float*)(ws + z.kt + z.tp + z.gates + z.ends);
     p.seg_blocks = z.seg_blocks;
     p.block_of[0] = p.seg_of[0] = 0;
     for (int s = 0; s < bt.n_seq; s++) {
@@ -944,7 +952,7 @@ extern "C" int32_t tsv_gdn_prefill(void* stream, const tsv_gdn_layer* layer, con
     if (done || !io->z || !bt.off[bt.n_seq]) return done;
     int group = 2;
     while (group * 8 < sh.dv) group *= 2;
-    const int64_t heads = (int64_t)bt.off[bt.n_seq] * sh.hv, wgs = (heads * group + 255) / 256;
+    const int64_t heads = (int64_t)bt.off[bt.n_seq] * sh.hv, wgs = std::min<int64_t>((heads * group + 255) / 256, 1 << 20);
     if (f16) hipLaunchKernelGGL((k_gdn_norm<true>), dim3((uint32_t)wgs), dim3(256), 0, st, sh, p.out, p.out_stride, (const uint16_t*)io->z, io->z_stride, heads, group);
     else hipLaunchKernelGGL((k_gdn_norm<false>), dim3((uint32_t)wgs), dim3(256), 0, st, sh, p.out, p.out_stride, (const uint16_t*)io->z, io->z_stride, heads, group);
     TSV_HIP(hipGetLastError());
