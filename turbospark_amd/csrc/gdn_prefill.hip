@@ -774,29 +774,24 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
 // ---- the gated norm, in place --------------------------------------------------------------------------------------------------------
 // v_dim / 8 of GROUP neighbouring lanes hold a head's row.
 template <bool F16>
-__global__ __launch_bounds__(256) void k_gdn_norm(GdnShape sh, uint16_t* out, int64_t out_stride, const uint16_t* z, int64_t z_stride, int64_t heads, int group) {
-    const int c = (threadIdx.x & (group - 1)) * 8, a_wg = 256 / group;
-    for (int64_t first = (int64_t)blockIdx.x * a_wg; first < heads; first += (int64_t)gridDim.x * a_wg) {
-        const int64_t at = first + threadIdx.x / group;
-        const int64_t row = heads <= INT32_MAX ? (int64_t)((uint32_t)at / (uint32_t)sh.hv) : at / sh.hv;
-        const bool in = at < heads && c < sh.dv;
-        const int h = (int)(at - row * sh.hv);
-        uint16_t* o = out + row * out_stride + h * sh.dv + c;
-        float x[8] = {}, y[8] = {}, sum = 0.0f;
-        if (in) {
-            row8_f32<F16>(*(const uint4*)o, x);
-            row8_f32<F16>(*(const uint4*)(z + row * z_stride + h * sh.dv + c), y);
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) sum = fmaf(x[e], x[e], sum);
-        for (int d = 1; d < group; d <<= 1) sum += __shfl_xor(sum, d);
-        if (in) {
-            const float f = rsqrtf(sum / (float)sh.dv + sh.norm_eps);
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] *= f * sh.norm[c + e] * silu_f32(y[e]);
-            *(uint4*)o = make_uint4(row_pair<F16>(x[0], x[1]), row_pair<F16>(x[2], x[3]), row_pair<F16>(x[4], x[5]), row_pair<F16>(x[6], x[7]));
-        }
+__global__ __launch_bounds__(256) void k_gdn_norm(GdnShape sh, uint16_t* out, int64_t out_stride, const uint16_t* z, int64_t z_stride, uint32_t heads, int group) {
+    const uint32_t at = (blockIdx.x * 256 + threadIdx.x) / group, row = at / sh.hv, h = at - row * sh.hv;
+    const int c = (threadIdx.x & (group - 1)) * 8;
+    const bool in = at < heads && c < sh.dv;
+    uint16_t* o = out + (int64_t)row * out_stride + h * sh.dv + c;
+    float x[8] = {}, y[8] = {}, sum = 0.0f;
+    if (in) {
+        row8_f32<F16>(*(const uint4*)o, x);
+        row8_f32<F16>(*(const uint4*)(z + (int64_t)row * z_stride + h * sh.dv + c), y);
     }
+#pragma unroll
+    for (int e = 0; e < 8; e++) sum = fmaf(x[e], x[e], sum);
+    for (int d = 1; d < group; d <<= 1) sum += __shfl_xor(sum, d);
+    if (!in) return;
+    const float f = rsqrtf(sum / (float)sh.dv + sh.norm_eps);
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = x[e] * f * sh.norm[c + e] * silu_f32(y[e]);
+    *(uint4*)o = make_uint4(row_pair<F16>(x[0], x[1]), row_pair<F16>(x[2], x[3]), row_pair<F16>(x[4], x[5]), row_pair<F16>(x[6], x[7]));
 }
 
 namespace {
@@ -952,9 +947,14 @@ extern "C" int32_t tsv_gdn_prefill(void* stream, const tsv_gdn_layer* layer, con
     if (done || !io->z || !bt.off[bt.n_seq]) return done;
     int group = 2;
     while (group * 8 < sh.dv) group *= 2;
-    const int64_t heads = (int64_t)bt.off[bt.n_seq] * sh.hv, wgs = std::min<int64_t>((heads * group + 255) / 256, 1 << 20);
-    if (f16) hipLaunchKernelGGL((k_gdn_norm<true>), dim3((uint32_t)wgs), dim3(256), 0, st, sh, p.out, p.out_stride, (const uint16_t*)io->z, io->z_stride, heads, group);
-    else hipLaunchKernelGGL((k_gdn_norm<false>), dim3((uint32_t)wgs), dim3(256), 0, st, sh, p.out, p.out_stride, (const uint16_t*)io->z, io->z_stride, heads, group);
+    const int rows = bt.off[bt.n_seq], at_once = (1 << 26) / sh.hv;  // (a launch has 2^32 threads at most)
+    for (int r = 0; r < rows; r += at_once) {
+        const uint32_t heads = (uint32_t)std::min(at_once, rows - r) * sh.hv, wgs = (uint32_t)(((uint64_t)heads * group + 255) / 256);
+        uint16_t* out = p.out + (int64_t)r * p.out_stride;
+        const uint16_t* gate = (const uint16_t*)io->z + (int64_t)r * io->z_stride;
+        if (f16) hipLaunchKernelGGL((k_gdn_norm<true>), dim3(wgs), dim3(256), 0, st, sh, out, p.out_stride, gate, io->z_stride, heads, group);
+        else hipLaunchKernelGGL((k_gdn_norm<false>), dim3(wgs), dim3(256), 0, st, sh, out, p.out_stride, gate, io->z_stride, heads, group);
+    }
     TSV_HIP(hipGetLastError());
     return TSV_OK;
 }
