@@ -109,4 +109,44 @@ __device__ __forceinline__ void wave_lds_fence() {
     __builtin_amdgcn_wave_barrier();
 }
 
+// (I + A)^-1 of a strictly lower 16 x 16 matrix by one wave, both in LDS with rows of a multiple of four floats: the 8 x 8 halves on the
+// diagonal row by row, a column a lane, both in the same instructions; then the block below, -T2 A21 T1, as two products of the f32
+// instruction, whose D layout is its B operand's when the contraction takes rows 4 gq + r in step r.  second: whether rows 8 to 15 hold anything.
+__device__ __forceinline__ void invert_lower16(const float* A, int as, float* T, int ts, int l16, int gq, bool second = true) {
+    const int b = l16 & 8;
+    const float* a = A + b * as + b;
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float v = i == (l16 & 7) ? 1.0f : 0.0f;
+#pragma unroll
+        for (int j = 0; j < i; j++) v = fmaf(-a[i * as + j], x[j], v);
+        x[i] = v;
+    }
+    if (gq < 2) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) T[((gq ? 8 - b : b) + i) * ts + l16] = gq ? 0.0f : x[i];
+    }
+    wave_lds_fence();
+    if (!second) return;
+    float4 r = *(const float4*)(A + l16 * as + 4 * gq);
+    if (l16 < 8 || gq > 1) r = make_float4(0, 0, 0, 0);
+    const float4 n = *(const float4*)(T + l16 * ts + 4 * gq);
+    gf4 t, p = {0, 0, 0, 0}, y = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 4; i++) t[i] = T[(4 * gq + i) * ts + l16];
+    p = mfma_f32(r.x, t[0], p);
+    p = mfma_f32(r.y, t[1], p);
+    p = mfma_f32(r.z, t[2], p);
+    p = mfma_f32(r.w, t[3], p);
+    y = mfma_f32(n.x, p[0], y);
+    y = mfma_f32(n.y, p[1], y);
+    y = mfma_f32(n.z, p[2], y);
+    y = mfma_f32(n.w, p[3], y);
+    if (gq > 1) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) T[(4 * gq + i) * ts + l16] = t[i] - y[i];
+    }
+}
+
 }  // namespace tsv

@@ -363,23 +363,7 @@ __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step(GdnShap
         }
         if (which == 0) {
             wave_lds_fence();
-            float x[16];  // column l16 of T, row after row
-#pragma unroll
-            for (int i = 0; i < 16; i++) x[i] = i == l16 ? 1.0f : 0.0f;
-#pragma unroll
-            for (int b = 0; b < 4; b++) {
-                if (4 * b >= m) break;
-#pragma unroll
-                for (int i = 4 * b; i < 4 * b + 4; i++) {
-                    float a[16];
-#pragma unroll
-                    for (int j = 0; j < i; j += 4) *(float4*)(a + j) = *(const float4*)(A + i * 20 + j);
-#pragma unroll
-                    for (int j = 0; j < i; j++) x[i] = fmaf(-a[j], x[j], x[i]);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 4; i++) T[(4 * i + gq) * 20 + l16] = gq == 0 ? x[4 * i] : gq == 1 ? x[4 * i + 1] : gq == 2 ? x[4 * i + 2] : x[4 * i + 3];
+            invert_lower16(A, 20, T, 20, l16, gq, m > 8);
         }
     }
     if (base == 0) {
