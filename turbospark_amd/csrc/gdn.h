@@ -74,6 +74,9 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
     lo = row_pair<false>(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u));
 }
 
+// a store that does not stay in the L2: it is on its way to memory while the kernel runs, not when it ends
+__device__ __forceinline__ void store_through(void* to, gf4 x) { __builtin_nontemporal_store(x, (gf4*)to); }
+
 __device__ __forceinline__ gf4 mfma_bf16(bf16x8 a, bf16x8 b, gf4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 __device__ __forceinline__ gf4 mfma_f32(float a, float b, gf4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 

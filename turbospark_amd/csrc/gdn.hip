@@ -11,7 +11,8 @@ namespace tsv {
 // A thread owns 8 neighbouring channels and walks a tile of rows, four at a time with the next four under way and the taps' rows in
 // registers: every row is read once, conv_width - 1 of them again per tile.  The k_dim / 8 threads of a head are neighbours in a wave
 // and sum its squares by lane moves.  Bound by memory (4 bytes a channel) and, close behind, by the exponential and the reciprocal of
-// each SiLU.  Tiles have 32 rows, or 4 where 32 would leave compute units without a workgroup.
+// each SiLU.  Tiles have 32 rows, or 4 where 32 would leave compute units without a workgroup.  8192 rows of 8192 channels: 57 us, 4.7
+// TB/s (60 where the rows stay in the L2 as they are stored); 299 rows of 1024: 4.8 us, the chain of loads.
 constexpr int CONV_THREADS = 256;
 
 struct ConvArgs {
@@ -105,7 +106,8 @@ __global__ __launch_bounds__(CONV_THREADS) void k_gdn_conv(GdnShape sh, GdnBatch
                 for (int e = 0; e < 8; e++) y[e] *= f;
             }
             if (r + i < rows)
-                *(uint4*)(out + (r + i) * p.out_stride) = make_uint4(row_pair<F16>(y[0], y[1]), row_pair<F16>(y[2], y[3]), row_pair<F16>(y[4], y[5]), row_pair<F16>(y[6], y[7]));
+                store_through(out + (r + i) * p.out_stride, __builtin_bit_cast(gf4, make_uint4(row_pair<F16>(y[0], y[1]), row_pair<F16>(y[2], y[3]),
+                                                                                             row_pair<F16>(y[4], y[5]), row_pair<F16>(y[6], y[7]))));
         }
 #pragma unroll
         for (int j = 0; j < 3; j++)
@@ -127,7 +129,8 @@ __global__ __launch_bounds__(CONV_THREADS) void k_gdn_conv(GdnShape sh, GdnBatch
 //     T = (I + A)^-1,  A_ij = beta_i D_ij k_i.k_j (j a strict ancestor of i),    P_ij = D_ij q_i.k_j (j an ancestor or i)
 // while the others go on to KS = k S, QS = q S (three bf16 products each: 2^-17, see split2).  Then, for all rows at once,
 // u = T beta (v - e^G KS), o = e^G QS + P u, and for final rows S <- e^G_end S + sum_i D_end,i k_i u_i (f32 matrix instructions).
-// With many sequences the state's bytes bound it, with one the chain of loads and three barriers.
+// With one sequence the chain of loads and three barriers bounds it (32 heads of 128, 5 rows: 9.0 us; 16-row trees of 4 sequences: 12.9
+// us), with many the state's bytes.
 // Operand order of the contraction over k_dim: lane group gq of the 16x16x32 instruction takes elements 4 gq .. + 3 of both
 // 16-wide halves of its 32, so that two neighbouring D tiles of the f32 update are exactly one B operand.
 
@@ -457,7 +460,8 @@ __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step(GdnShap
 
 // The same for one row a sequence, plain decoding: u = beta (v - e^g k S), o = e^g q S + (q.k) u, S <- e^g S + k u^T need no
 // 16 x 16 matrices and no operand fragments, and the products with the state are f32 dot products of a lane's k_dim / 4 values, summed
-// over the four lanes of a channel.  Two barriers.
+// over the four lanes of a channel.  Two barriers.  32 heads of 128: one sequence 7.3 us, 128 sequences 124 us for 537 MB of state (4.3
+// TB/s; 132 with stores that do not stay in the L2, 129 to 140 with such loads too).
 template <int DK, bool F16, int THREADS>
 __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step_one(GdnShape sh, StepArgs p, GdnBatch bt) {
     __shared__ float4 q4[DK / 4], k4[DK / 4];
@@ -573,8 +577,12 @@ __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step_one(Gdn
 // ---- accepted rows into the state -----------------------------------------------------------------------------------------------
 // S <- e^{g_1 + .. + g_n} S + sum_i e^{g_{i+1} + .. + g_n} k_i u_i^T over the kept path.  A thread keeps four state values of
 // COMMIT_PIECES neighbouring value channels; the path, the same for a workgroup, goes through scalar registers, and from it four rows'
-// k and u at a time are under way.  One pass over the state, which is what bounds it.  The last workgroups of a (sequence, layer)
-// move the ring's rows: slot i takes the row of slot path[i] >= i, in ascending order by one thread.
+// k and u at a time are under way.  One pass over the state, which is what bounds it: three rows of one sequence in 24 layers of 32 heads
+// of 128, 101 MB of state, 19 us (5.2 TB/s; 26 where the stores stay in the L2); trees of 16 rows of 32 sequences, 134 MB, 25 us (31).
+// (Steps of all those layers right behind it take 0.4 us more each, which find the state in the L2 else; a model's products between them
+// would have emptied it.)
+// The last workgroups of a (sequence, layer) move the ring's rows: slot i takes the row of slot path[i] >= i, in ascending order by one
+// thread.
 constexpr int COMMIT_THREADS = 256, COMMIT_PIECES = 4;
 
 struct CommitArgs {
@@ -686,7 +694,7 @@ __global__ __launch_bounds__(COMMIT_THREADS) void k_gdn_commit(GdnShape sh, Comm
         }
     }
 #pragma unroll
-    for (int i = 0; i < COMMIT_PIECES; i++) *(float4*)(p.state_out + at + i * DK) = S[i];
+    for (int i = 0; i < COMMIT_PIECES; i++) store_through(p.state_out + at + i * DK, __builtin_bit_cast(gf4, S[i]));
 }
 
 // ---- arguments ----------------------------------------------------------------------------------------------------------------

@@ -308,8 +308,8 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
 // SIMD, make the output rows from the same LDS (q S behind the first barrier, P u behind the third) and hand the others v, transposed,
 // and the decays through LDS: a load or store of any width holds the CU's address unit for 16 cycles, which bounds a block (12 and 9 of
 // them a wave here), so two-byte ones are taken together.  Everything a block reads is asked for one block ahead, into the registers
-// just used: the scheduling fences keep the compiler from asking earlier, which would take copies and, with them, waits.  The column tiles of a head read the same k, q, T and P: workgroups are numbered so that they share an
-// XCD's L2.
+// just used: the scheduling fences keep the compiler from asking earlier, which would take copies and, with them, waits.  The column
+// tiles of a head read the same k, q, T and P: workgroups are numbered so that they share an XCD's L2.
 // Where few heads leave most of the chip idle a sequence is cut into segments.  A block takes every column of the state alike, S -> M S + c
 // with M the same for all, so a first launch (ENDS) walks all segments but the last at once, from nothing with the rows' v and from the
 // unit matrix with v = 0; the walk of segment n then begins with n products M S + c of its own 16 NT columns.
