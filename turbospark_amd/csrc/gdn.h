@@ -95,15 +95,25 @@ __device__ __forceinline__ float decay_of(float a_log, float x) {
     return -__expf(a_log) * fmaf(2.0f * s, y, fmaxf(x, 0.0f));
 }
 
-// The sum of x over LANES neighbouring lanes (8, 16 or 32), in all of them: lanes 1, 2, 7 - i and 15 - i apart, without LDS.
+// The sum of x over LANES neighbouring lanes (4, 8, 16 or 32), in all of them: lanes 1, 2, 7 - i and 15 - i apart, without LDS.
 template <int LANES>
 __device__ __forceinline__ float sum_lanes(float x) {
-    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xF, 0xF, true));   // quad_perm 1 0 3 2
-    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xF, 0xF, true));   // quad_perm 2 3 0 1
-    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xF, 0xF, true));  // row_half_mirror
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xF, 0xF, true));  // quad_perm 1 0 3 2
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xF, 0xF, true));  // quad_perm 2 3 0 1
+    if constexpr (LANES >= 8) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xF, 0xF, true));   // row_half_mirror
     if constexpr (LANES >= 16) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xF, 0xF, true));  // row_mirror
     if constexpr (LANES >= 32) x += __shfl_xor(x, 16);
     return x;
+}
+
+// Two values to be summed over pairs of lanes 16 or 32 apart: the sum of x in the lower lane of the pair, that of y in the upper.
+__device__ __forceinline__ float lane_pairs_by_16(float x, float y) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ float lane_pairs_by_32(float x, float y) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(y), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
 // orders a wave's own LDS writes before its own later reads, where no other wave is involved

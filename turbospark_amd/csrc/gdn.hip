@@ -459,9 +459,53 @@ __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step(GdnShap
 }
 
 // The same for one row a sequence, plain decoding: u = beta (v - e^g k S), o = e^g q S + (q.k) u, S <- e^g S + k u^T need no
-// 16 x 16 matrices and no operand fragments, and the products with the state are f32 dot products of a lane's k_dim / 4 values, summed
-// over the four lanes of a channel.  Two barriers.  32 heads of 128: one sequence 7.3 us, 128 sequences 124 us for 537 MB of state (4.3
-// TB/s; 132 with stores that do not stay in the L2, 129 to 140 with such loads too).
+// 16 x 16 matrices and no operand fragments; the products with the state are f32 dot products over the k_dim / 4 neighbouring lanes of a
+// channel.  A wave's 16 channels x k_dim are one run of memory, taken 1 KiB an instruction: whole lines in and out (lanes that held k_dim
+// / 4 values of one channel, 64 bytes of 16 lines an instruction, took 7.4 us where this takes 5.2, and 124 where this takes 101).  Two
+// barriers.  32 heads of 128: one sequence 5.2 us, 128 sequences 101 us for 537 MB of state (5.3 TB/s; 107 with stores that stay in the
+// L2).
+
+// sums over the DK / 4 lanes of each of the NT x 256 / DK channels that the lanes' x belong to: x[0 .. 3] become the sums of channels
+// 4 j + one_row_channel, the same in all lanes of a row of sixteen
+template <int DK>
+__device__ __forceinline__ void one_row_sums(float* x) {
+    if constexpr (DK == 256) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = lane_pairs_by_32(x[2 * i], x[2 * i + 1]);
+    }
+    if constexpr (DK >= 128) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = lane_pairs_by_16(x[2 * i], x[2 * i + 1]);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = sum_lanes<16>(x[i]);
+}
+template <int DK>
+__device__ __forceinline__ int one_row_channel(int row) {
+    return DK == 64 ? row : 2 * (row & 1) + (row >> 1);
+}
+// the other way: u, which lane j of every four holds for channel 4 j + one_row_channel, to the channels of x[NT]
+template <int DK>
+__device__ __forceinline__ void one_row_spread(float u, float* x) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const int v = __float_as_int(u);
+        const float w = __int_as_float(j == 0   ? __builtin_amdgcn_update_dpp(0, v, 0x00, 0xF, 0xF, true)
+                                       : j == 1 ? __builtin_amdgcn_update_dpp(0, v, 0x55, 0xF, 0xF, true)
+                                       : j == 2 ? __builtin_amdgcn_update_dpp(0, v, 0xAA, 0xF, 0xF, true)
+                                                : __builtin_amdgcn_update_dpp(0, v, 0xFF, 0xF, 0xF, true));
+        if constexpr (DK == 64) x[j] = w;
+        if constexpr (DK == 128) {
+            const float2 r = lanes_by_16(w);
+            x[2 * j] = r.x, x[2 * j + 1] = r.y;
+        }
+        if constexpr (DK == 256) {
+            const float2 r = lanes_by_16(w), a = lanes_by_32(r.x), b = lanes_by_32(r.y);
+            x[4 * j] = a.x, x[4 * j + 1] = a.y, x[4 * j + 2] = b.x, x[4 * j + 3] = b.y;
+        }
+    }
+}
+
 template <int DK, bool F16, int THREADS>
 __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step_one(GdnShape sh, StepArgs p, GdnBatch bt) {
     __shared__ float4 q4[DK / 4], k4[DK / 4];
@@ -471,21 +515,21 @@ __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step_one(Gdn
                  "s"(p.record), "s"(p.out), "s"(p.out_stride), "s"(p.total_rows), "s"(bt.base));
     const int hk = blockIdx.y, h = hk * sh.rep + blockIdx.x, s = blockIdx.z, dv = sh.dv, tid = threadIdx.x;
     const int row = bt.off[s], m = bt.off[s + 1] - row, taps = sh.taps;
-    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, gq = lane >> 4, waves = dv >> 4;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), waves = dv >> 4;
     const int64_t base = bt.base[s];
-    const size_t at = ((size_t)s * sh.hv + h) * dv * DK + (size_t)(16 * wave + l16) * DK + 4 * gq;
+    const size_t at = ((size_t)s * sh.hv + h) * dv * DK + (size_t)(16 * wave * DK + 4 * lane);
     constexpr int NT = DK / 16;
     float4 S[NT];
 #pragma unroll
-    for (int t = 0; t < NT; t++) S[t] = *(const float4*)(p.state_in + at + 16 * t);
+    for (int t = 0; t < NT; t++) S[t] = *(const float4*)(p.state_in + at + 256 * t);
     if (m <= 0) {  // no row: the state stays
         if (p.state_out) {
 #pragma unroll
-            for (int t = 0; t < NT; t++) *(float4*)(p.state_out + at + 16 * t) = base == 0 ? make_float4(0, 0, 0, 0) : S[t];
+            for (int t = 0; t < NT; t++) *(float4*)(p.state_out + at + 256 * t) = base == 0 ? make_float4(0, 0, 0, 0) : S[t];
         }
         return;
     }
-    const int col = 16 * wave + l16;  // this lane's value channel
+    const int col = 16 * wave + 4 * (lane & 3) + one_row_channel<DK>(lane >> 4);  // the value channel whose u and o this lane makes
     uint16_t zr = 0;
     float nw = 0.0f;
     if (p.z) {
@@ -532,26 +576,28 @@ __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step_one(Gdn
 #pragma unroll
         for (int t = 0; t < NT; t++) S[t] = make_float4(0, 0, 0, 0);
     }
-    float ks = 0.0f, qs = 0.0f, qk = 0.0f;
+    const float4 k = k4[lane & (DK / 4 - 1)], q = q4[lane & (DK / 4 - 1)];
+    float ks4[NT], qs4[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-        const float4 k = k4[4 * t + gq], q = q4[4 * t + gq];
-        ks = fmaf(k.x, S[t].x, fmaf(k.y, S[t].y, fmaf(k.z, S[t].z, fmaf(k.w, S[t].w, ks))));
-        qs = fmaf(q.x, S[t].x, fmaf(q.y, S[t].y, fmaf(q.z, S[t].z, fmaf(q.w, S[t].w, qs))));
-        qk = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, qk))));
+        ks4[t] = fmaf(k.x, S[t].x, fmaf(k.y, S[t].y, fmaf(k.z, S[t].z, k.w * S[t].w)));
+        qs4[t] = fmaf(q.x, S[t].x, fmaf(q.y, S[t].y, fmaf(q.z, S[t].z, q.w * S[t].w)));
     }
+    one_row_sums<DK>(ks4);
+    one_row_sums<DK>(qs4);
     float2 r;
-    r = lanes_by_16(ks), ks = r.x + r.y;
-    r = lanes_by_32(ks), ks = r.x + r.y;
-    r = lanes_by_16(qs), qs = r.x + r.y;
-    r = lanes_by_32(qs), qs = r.x + r.y;
-    r = lanes_by_16(qk), qk = r.x + r.y;
-    r = lanes_by_32(qk), qk = r.x + r.y;
+    float qk = sum_lanes<16>(fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, q.w * k.w))));
+    if constexpr (DK >= 128) r = lanes_by_16(qk), qk = r.x + r.y;
+    if constexpr (DK == 256) r = lanes_by_32(qk), qk = r.x + r.y;
+    const float ks = lane & 2 ? (lane & 1 ? ks4[3] : ks4[2]) : lane & 1 ? ks4[1] : ks4[0];
+    const float qs = lane & 2 ? (lane & 1 ? qs4[3] : qs4[2]) : lane & 1 ? qs4[1] : qs4[0];
     const float e = gate[0], u = gate[1] * fmaf(-e, ks, vv[col]);
     float o = sh.scale * fmaf(qk, u, e * qs);
     if (p.z) {
-        const float q = sum_lanes<16>(o * o);
-        if (lane == 0) red[wave] = q;
+        float sq = sum_lanes<4>(o * o);
+        r = lanes_by_16(sq), sq = r.x + r.y;
+        r = lanes_by_32(sq), sq = r.x + r.y;
+        if (lane == 0) red[wave] = sq;
         __syncthreads();
         float sum = 0.0f;
 #pragma unroll
@@ -561,16 +607,16 @@ __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step_one(Gdn
         }
         o *= rsqrtf(sum / (float)dv + sh.norm_eps) * nw * silu_f32(row_f32<F16>(zr));
     }
-    if (gq == 0) {
+    if ((lane & 12) == 0) {
         p.out[(int64_t)row * p.out_stride + h * dv + col] = row_bits<F16>(o);
         if (p.record) p.record[((size_t)row * sh.hv + h) * dv + col] = u;
     }
     if (p.state_out) {
+float us[NT];
+        one_row_spread<DK>(u, us);
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const float4 k = k4[4 * t + gq];
-            *(float4*)(p.state_out + at + 16 * t) = make_float4(fmaf(u, k.x, e * S[t].x), fmaf(u, k.y, e * S[t].y), fmaf(u, k.z, e * S[t].z), fmaf(u, k.w, e * S[t].w));
-        }
+        for (int t = 0; t < NT; t++)
+            store_through(p.state_out + at + 256 * t, gf4{fmaf(us[t], k.x, e * S[t].x), fmaf(us[t], k.y, e * S[t].y), fmaf(us[t], k.z, e * S[t].z), fmaf(us[t], k.w, e * S[t].w)});
     }
 }
 
