@@ -313,6 +313,8 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
 // Where few heads leave most of the chip idle a sequence is cut into segments.  A block takes every column of the state alike, S -> M S + c
 // with M the same for all, so a first launch (ENDS) walks all segments but the last at once, from nothing with the rows' v and from the
 // unit matrix with v = 0; the walk of segment n then begins with n products M S + c of its own 16 NT columns.
+// 8192 rows of 32 heads of 128, one column tile on each compute unit: 185 us, 1.4 us a block, in which the three hand-overs through LDS
+// follow each other and the address unit is busy for two thirds; the bytes would take 35 us, the products 20.
 #define GDN_FENCE __builtin_amdgcn_sched_barrier(0)
 // all loads have arrived, and the compiler knows: what is under way before a loop would else count in every wait inside it
 #define GDN_ARRIVED                            \
@@ -762,7 +764,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
 #undef GDN_ARRIVED
 
 // ---- the gated norm, in place --------------------------------------------------------------------------------------------------------
-// v_dim / 8 of GROUP neighbouring lanes hold a head's row.
+// v_dim / 8 of GROUP neighbouring lanes hold a head's row.  Bound by memory: 8192 rows of 32 heads of 128, 201 MB, 35 us (5.7 TB/s).
 template <bool F16>
 __global__ __launch_bounds__(256) void k_gdn_norm(GdnShape sh, uint16_t* out, int64_t out_stride, const uint16_t* z, int64_t z_stride, uint32_t heads, int group) {
     const uint32_t at = (blockIdx.x * 256 + threadIdx.x) / group, row = at / sh.hv, h = at - row * sh.hv;
@@ -790,8 +792,8 @@ int64_t blocks_of(const GdnBatch& bt, int s) { return (bt.off[s + 1] - bt.off[s]
 
 // How many blocks a segment has, INT32_MAX: whole sequences.  In segments a sequence's columns are walked twice and the k_dim columns of the
 // unit matrix once, so that it pays where at most a quarter of the compute units would have a workgroup: 32768 rows of 8 heads of 128
-// (64 column tiles) took 605 us whole, 360 in 4 segments, 319 in 8, 360 in 16.  Segments of fewer than 8 blocks gain nothing over
-// what putting them together takes (1.5 us each).
+// (64 column tiles) take 596 us whole, 338 in 4 segments (157 for M and c, 181), 290 in 8 (157 and 133), 331 in 16 (163 and 168).
+// Segments of fewer than 8 blocks gain nothing over what putting them together takes (2.5 us each).
 int segment_blocks(const GdnShape& sh, const GdnBatch& bt) {
     int64_t longest = 0;
     for (int s = 0; s < bt.n_seq; s++) longest = std::max(longest, blocks_of(bt, s));
@@ -858,7 +860,7 @@ int launch_prefill(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, Prefi
         if (rc) return rc;
     }
     // Two column tiles a workgroup where that still gives every compute unit one: they share what a block reads (6 sequences, 32 heads of
-    // 128: 70 us against 100); else one, for the shorter way through a block (8192 rows, 32 heads: 189 us against 219).  k_dim 256 has no
+    // 128: 72 us against 106); else one, for the shorter way through a block (8192 rows, 32 heads: 185 us against 208).  k_dim 256 has no
     // registers for two.
     if (p.seg_of[bt.n_seq] > bt.n_seq) {
         int rc;
