@@ -429,6 +429,32 @@ def test_final_rows(hk, hv, dk, dv, dtype, lengths, base, in_place):
     p.check(final="in place" if in_place else "new")
 
 
+@pytest.mark.parametrize("lengths,base", [([1, 1], [0, 9]), ([4, 1], [70, 0])])
+@pytest.mark.parametrize("final,record", [(True, True), (False, False)])
+def test_new_state_and_record_or_neither(lengths, base, final, record):
+    rng = np.random.default_rng(8)
+    p = Step(rng, Layer(rng, 2, 4, 128, 64, 4, BF), lengths, base, gated=True)
+    if final:
+        p.io.state_out = p.dnew.ptr
+    if record:
+        p.io.record = p.record.ptr
+    before = p.din.get()
+    p.ly.gpu.step(p.batch, p.io)
+    p.check(final="new" if final else None, record=record)
+    assert np.array_equal(p.din.get().view(np.uint32), before.view(np.uint32))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_wider_passes_behind_narrow_ones(dtype):
+    """The widest heads, more shared memory from pass to pass."""
+    for rows in (2, 11, 14, 16):
+        rng = np.random.default_rng(rows)
+        p = Step(rng, Layer(rng, 1, 1, 256, 256, 4, dtype), [rows], [3])
+        p.io.record = p.record.ptr
+        p.ly.gpu.step(p.batch, p.io)
+        p.check(record=True)
+
+
 @pytest.mark.parametrize("taps", [1, 2, 3])
 def test_fewer_taps_through_a_tree(taps):
     rng = np.random.default_rng(taps)

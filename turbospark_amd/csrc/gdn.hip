@@ -833,9 +833,10 @@ int launch_step(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, const St
         TSV_HIP(hipGetLastError());
         return TSV_OK;
     }
-    const size_t lds = sizeof(float) * (size_t)(step_lds<DK> + p.max_rows * (DK + sh.dv) + 256);
-    static OncePerDevice once;
-    const int rc = allow_lds((const void*)k_gdn_step<DK, F16, THREADS>, lds, once);
+    auto bytes = [](int rows, int dv) { return sizeof(float) * (size_t)(step_lds<DK> + rows * (DK + dv) + 256); };
+    const size_t lds = bytes(p.max_rows, sh.dv);
+    static OncePerDevice once;  // (asked for once: for the most that a call can need)
+    const int rc = allow_lds((const void*)k_gdn_step<DK, F16, THREADS>, bytes(TSV_MAX_ROWS, THREADS / 4), once);
     if (rc) return rc;
     hipLaunchKernelGGL((k_gdn_step<DK, F16, THREADS>), dim3(sh.rep, sh.hk, bt.n_seq), dim3(64 * waves), lds, st, sh, p, bt);
     TSV_HIP(hipGetLastError());
