@@ -494,13 +494,15 @@ typedef struct {
 } tsv_gdn_batch;
 
 /* The convolution's part for prompts: out gets channels values a row (unit q, unit k, v) in the rows' type, g and beta (f32,
- * rows x n_v_heads) the decays and betas; the last conv_width - 1 rows of every sequence go to its ring. */
+ * rows x n_v_heads) the decays and betas; the last conv_width - 1 rows of every sequence go to its ring.  Slots of ring_out that
+ * no row goes to are left as they are (ring_out other than ring_in: a pass that can be made again from the same rings). */
 typedef struct {
     const void* qkv;
     int64_t qkv_stride;
     const void *a, *b;   /* n_v_heads a row */
     int64_t gate_stride; /* of a and b; any value >= n_v_heads */
-    void* ring;
+    const void* ring_in;
+    void* ring_out;
     void* out;
     int64_t out_stride;
     float *g, *beta;

@@ -29,7 +29,7 @@ def _batch(offsets=(0, 3), **over):
 
 CH = 2 * 2 * 64 + 4 * 32
 IO = {
-    "conv": lambda: ffi.GdnConv(qkv=P, qkv_stride=CH, a=P, b=P, gate_stride=4, ring=P, out=2 * P, out_stride=CH, g=P, beta=P),
+    "conv": lambda: ffi.GdnConv(qkv=P, qkv_stride=CH, a=P, b=P, gate_stride=4, ring_in=P, ring_out=P, out=2 * P, out_stride=CH, g=P, beta=P),
     "prefill": lambda: ffi.GdnPrefill(q=P, k=P, v=P, q_stride=128, k_stride=128, v_stride=128, g=P, beta=P, z=P, z_stride=128,
                                       state_in=P, state_out=P, out=2 * P, out_stride=128, workspace=P, workspace_bytes=1 << 30),
     "step": lambda: ffi.GdnStep(qkv=P, qkv_stride=CH, a=P, b=P, gate_stride=4, z=P, z_stride=128, ring=P, state_in=P, state_out=P,
@@ -67,7 +67,8 @@ def test_descriptions_are_refused_by_name(what):
 
 @pytest.mark.parametrize("what,fields", [
     ("conv", dict(qkv=None)), ("conv", dict(qkv=P + 8)), ("conv", dict(qkv_stride=CH - 8)), ("conv", dict(qkv_stride=CH + 4)),
-    ("conv", dict(out=P)), ("conv", dict(out_stride=8)), ("conv", dict(ring=None)), ("conv", dict(ring=P + 2)), ("conv", dict(gate_stride=3)),
+    ("conv", dict(out=P)), ("conv", dict(out_stride=8)), ("conv", dict(ring_in=None)), ("conv", dict(ring_out=None)),
+    ("conv", dict(ring_in=P + 2)), ("conv", dict(ring_out=P + 2)), ("conv", dict(ring_out=P + 64)), ("conv", dict(gate_stride=3)),
     ("conv", dict(a=None)), ("conv", dict(g=None)), ("conv", dict(beta=None)),
     ("prefill", dict(q=None)), ("prefill", dict(k=P + 2)), ("prefill", dict(v_stride=120)), ("prefill", dict(out=P)),
     ("prefill", dict(state_in=None)), ("prefill", dict(state_out=P + 64)), ("prefill", dict(workspace=None)),
@@ -119,5 +120,5 @@ def test_sizes_of_workspace_and_record():
 
 def test_struct_layouts_match_the_header():
     assert C.sizeof(ffi.GdnLayer) == 9 * 4 + 4 + 4 * 8 and C.sizeof(ffi.GdnBatch) == 4 * 8
-    assert (C.sizeof(ffi.GdnConv), C.sizeof(ffi.GdnPrefill), C.sizeof(ffi.GdnStep), C.sizeof(ffi.GdnCommit)) == (80, 128, 104, 80)
+    assert (C.sizeof(ffi.GdnConv), C.sizeof(ffi.GdnPrefill), C.sizeof(ffi.GdnStep), C.sizeof(ffi.GdnCommit)) == (88, 128, 104, 80)
     assert np.dtype(np.int32).itemsize * 28 == C.sizeof(ffi.RoundResultC)

@@ -20,7 +20,8 @@ struct ConvArgs {
     int64_t qkv_stride;
     const uint16_t *a, *b;
     int64_t gate_stride;
-    uint16_t* ring;
+    const uint16_t* ring_in;
+    uint16_t* ring_out;
     uint16_t* out;
     int64_t out_stride;
     float *g, *beta;
@@ -69,14 +70,14 @@ __global__ __launch_bounds__(CONV_THREADS) void k_gdn_conv(GdnShape sh, GdnBatch
 #pragma unroll
             for (int e = 0; e < 8; e++) w[j][e] = j < taps ? sh.conv[(int64_t)(c + e) * taps + taps - 1 - j] : 0.0f;
     }
-    uint16_t* ring = p.ring + (int64_t)s * TSV_GDN_RING * sh.channels + c;
+    const int64_t ring = (int64_t)s * TSV_GDN_RING * sh.channels + c;
     const int64_t base = r0 == 0 ? bt.base[s] : 0;
 #pragma unroll
     for (int j = 1; j < 4; j++) {
         uint4 u = make_uint4(0, 0, 0, 0);
         if (j < taps) {
             if (r0 - j >= 0) u = *(const uint4*)(in - j * p.qkv_stride);
-            else if (base - j >= 0) u = *(const uint4*)(ring + ((base - j) & (TSV_GDN_RING - 1)) * sh.channels);
+            else if (base - j >= 0) u = *(const uint4*)(p.ring_in + ring + ((base - j) & (TSV_GDN_RING - 1)) * sh.channels);
         }
         row8_f32<F16>(u, x[3 - j]);
     }
@@ -117,7 +118,7 @@ __global__ __launch_bounds__(CONV_THREADS) void k_gdn_conv(GdnShape sh, GdnBatch
     // the ring's new rows, by the thread that has read the old ones of these channels
     if (r0 == 0)
         for (int j = 1; j < taps && j <= n; j++)
-            *(uint4*)(ring + ((base + n - j) & (TSV_GDN_RING - 1)) * sh.channels) = *(const uint4*)(p.qkv + (int64_t)(first + n - j) * p.qkv_stride + c);
+            *(uint4*)(p.ring_out + ring + ((base + n - j) & (TSV_GDN_RING - 1)) * sh.channels) = *(const uint4*)(p.qkv + (int64_t)(first + n - j) * p.qkv_stride + c);
 }
 
 // ---- the step of a few rows -------------------------------------------------------------------------------------------------
@@ -866,19 +867,21 @@ extern "C" int32_t tsv_gdn_conv(void* stream, const tsv_gdn_layer* layer, const 
     GdnBatch bt;
     const int rc = gdn_check(who, stream, layer, batch, 0, &sh, &bt);
     if (rc) return rc;
-    if (!io || !io->a || !io->b || !io->ring || !io->g || !io->beta || !sh.conv || !sh.a_log || !sh.dt_bias) return gdn_refuse(who, "null argument");
+    if (!io || !io->a || !io->b || !io->ring_in || !io->ring_out || !io->g || !io->beta || !sh.conv || !sh.a_log || !sh.dt_bias) return gdn_refuse(who, "null argument");
     if (batch->parent) return gdn_refuse(who, "prompt rows are chains");
-    if (!gdn_rows_ok(io->qkv, io->qkv_stride, sh.channels) || !gdn_rows_ok(io->out, io->out_stride, sh.channels) || ((uintptr_t)io->ring & 15) ||
+    if (!gdn_rows_ok(io->qkv, io->qkv_stride, sh.channels) || !gdn_rows_ok(io->out, io->out_stride, sh.channels) || ((uintptr_t)io->ring_in & 15) || ((uintptr_t)io->ring_out & 15) ||
         io->gate_stride < sh.hv || ((uintptr_t)io->g & 3) || ((uintptr_t)io->beta & 3))
         return gdn_refuse(who, "rows, rings and strides: 16-byte aligned, multiples of 8, as wide as a row");
     if (io->out == io->qkv) return gdn_refuse(who, "out may not be the input rows");
+    if (gdn_overlap(io->ring_in, io->ring_out, 2 * (size_t)bt.n_seq * TSV_GDN_RING * sh.channels)) return gdn_refuse(who, "ring_out overlaps ring_in");
     ConvArgs p;
     p.qkv = (const uint16_t*)io->qkv;
     p.qkv_stride = io->qkv_stride;
     p.a = (const uint16_t*)io->a;
     p.b = (const uint16_t*)io->b;
     p.gate_stride = io->gate_stride;
-    p.ring = (uint16_t*)io->ring;
+    p.ring_in = (const uint16_t*)io->ring_in;
+    p.ring_out = (uint16_t*)io->ring_out;
     p.out = (uint16_t*)io->out;
     p.out_stride = io->out_stride;
     p.g = io->g;

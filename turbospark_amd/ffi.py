@@ -235,7 +235,8 @@ class GdnBatch(C.Structure):
 class GdnConv(C.Structure):
     """tsv_gdn_conv_io: device addresses, strides in elements."""
     _fields_ = [("qkv", C.c_void_p), ("qkv_stride", C.c_int64), ("a", C.c_void_p), ("b", C.c_void_p), ("gate_stride", C.c_int64),
-                ("ring", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_int64), ("g", C.c_void_p), ("beta", C.c_void_p)]
+                ("ring_in", C.c_void_p), ("ring_out", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_int64), ("g", C.c_void_p),
+                ("beta", C.c_void_p)]
 
 
 class GdnPrefill(C.Structure):
