@@ -143,7 +143,6 @@ def prepare(case, seed):
     if case["what"] == "conv":
         st["out"] = torch.empty((T, C), device=dev, dtype=dt)
         st["g"], st["beta"] = (torch.empty((T, hv), device=dev) for _ in range(2))
-        st["ring_out"] = st["ring"].clone()
     if case["what"] == "prefill":
         # rows as the convolution leaves them: q and k of unit length with a part that all rows share, v behind SiLU
         unit = lambda x: x / x.norm(dim=-1, keepdim=True)  # noqa: E731
@@ -219,7 +218,7 @@ def _plan(st):
     gate = dict(z=at("z"), z_stride=st["z"].stride(0)) if "z" in st and c["gated"] else {}
     if c["what"] == "conv":
         st["io"] = ts.GdnConv(qkv=at("qkv"), qkv_stride=st["qkv"].stride(0), a=at("a"), b=at("b"), gate_stride=st["a"].stride(0),
-                              ring_in=at("ring"), ring_out=at("ring_out"), out=at("out"), out_stride=st["out"].stride(0), g=at("g"), beta=at("beta"))
+                              ring=at("ring"), out=at("out"), out_stride=st["out"].stride(0), g=at("g"), beta=at("beta"))
     elif c["what"] == "prefill":
         st["workspace"] = torch.empty((st["layer"].prefill_workspace(st["batch"]),), device="cuda", dtype=torch.uint8)
         st["io"] = ts.GdnPrefill(q=at("qkv"), k=at("qkv") + 2 * kd, v=at("qkv") + 4 * kd, q_stride=st["qkv"].stride(0),
@@ -248,7 +247,7 @@ def _stream():
 
 def _own_conv(st):
     st["layer"].conv(st["batch"], st["io"], _stream())
-    return dict(rows=st["out"], g=st["g"], beta=st["beta"], ring=st["ring_out"])
+    return dict(rows=st["out"], g=st["g"], beta=st["beta"], ring=st["ring"])
 
 
 def _own_prefill(st):
