@@ -122,3 +122,21 @@ def test_struct_layouts_match_the_header():
     assert C.sizeof(ffi.GdnLayer) == 9 * 4 + 4 + 4 * 8 and C.sizeof(ffi.GdnBatch) == 4 * 8
     assert (C.sizeof(ffi.GdnConv), C.sizeof(ffi.GdnPrefill), C.sizeof(ffi.GdnStep), C.sizeof(ffi.GdnCommit)) == (88, 128, 104, 80)
     assert np.dtype(np.int32).itemsize * 28 == C.sizeof(ffi.RoundResultC)
+
+
+def test_one_ring_stands_for_both():
+    """A convolution that updates its ring in place names it once; what names one and both at once is refused."""
+    io = ffi.GdnConv(qkv=P, ring=3 * P, out=2 * P)
+    assert io.ring_in == io.ring_out == io.ring == 3 * P and io.qkv == P and io.out == 2 * P
+    io.ring = 4 * P
+    assert io.ring_in == io.ring_out == 4 * P
+    io.ring_out = 5 * P
+    assert io.ring is None and io.ring_in == 4 * P
+    for twice in (dict(ring_in=P), dict(ring_out=P)):
+        with pytest.raises(TypeError):
+            ffi.GdnConv(ring=P, **twice)
+    whole = IO["conv"]()
+    whole.ring = P + 2
+    assert _call("conv", _layer(), _batch(), whole) == INVALID and "rings" in ffi.last_error()
+    whole.ring = None
+    assert _call("conv", _layer(), _batch(), whole) == INVALID and "null" in ffi.last_error()

@@ -233,10 +233,25 @@ class GdnBatch(C.Structure):
 
 
 class GdnConv(C.Structure):
-    """tsv_gdn_conv_io: device addresses, strides in elements."""
+    """tsv_gdn_conv_io: device addresses, strides in elements.  `ring` stands for ring_in and ring_out, a ring that is updated in place."""
     _fields_ = [("qkv", C.c_void_p), ("qkv_stride", C.c_int64), ("a", C.c_void_p), ("b", C.c_void_p), ("gate_stride", C.c_int64),
                 ("ring_in", C.c_void_p), ("ring_out", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_int64), ("g", C.c_void_p),
                 ("beta", C.c_void_p)]
+
+    def __init__(self, *args, ring=None, **fields):
+        if ring is not None and ("ring_in" in fields or "ring_out" in fields):
+            raise TypeError("ring, or ring_in and ring_out")
+        super().__init__(*args, **fields)
+        if ring is not None:
+            self.ring = ring
+
+    @property
+    def ring(self):
+        return self.ring_in if self.ring_in == self.ring_out else None
+
+    @ring.setter
+    def ring(self, address):
+        self.ring_in = self.ring_out = address
 
 
 class GdnPrefill(C.Structure):
