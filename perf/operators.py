@@ -217,8 +217,11 @@ def _plan(st):
     st["batch"] = st["layer"].batch(st["offsets"], at("base"), at("parent") if c["what"] == "step" and c["tree"] else None)
     gate = dict(z=at("z"), z_stride=st["z"].stride(0)) if "z" in st and c["gated"] else {}
     if c["what"] == "conv":
+        # a pass is made again from the same position: it reads the ring as it was and writes a copy, or the last rows of 30 to 34 (and 62 to 66, ..)
+        # would lie where the first ones' predecessors are read
+        st["ring_before"], st["ring"] = st["ring"], st["ring"].clone()
         st["io"] = ts.GdnConv(qkv=at("qkv"), qkv_stride=st["qkv"].stride(0), a=at("a"), b=at("b"), gate_stride=st["a"].stride(0),
-                              ring=at("ring"), out=at("out"), out_stride=st["out"].stride(0), g=at("g"), beta=at("beta"))
+                              ring_in=at("ring_before"), ring_out=at("ring"), out=at("out"), out_stride=st["out"].stride(0), g=at("g"), beta=at("beta"))
     elif c["what"] == "prefill":
         st["workspace"] = torch.empty((st["layer"].prefill_workspace(st["batch"]),), device="cuda", dtype=torch.uint8)
         st["io"] = ts.GdnPrefill(q=at("qkv"), k=at("qkv") + 2 * kd, v=at("qkv") + 4 * kd, q_stride=st["qkv"].stride(0),
