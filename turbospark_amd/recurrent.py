@@ -15,9 +15,12 @@ class Batch:
     row, None: chains) are device addresses."""
 
     def __init__(self, offsets, base, parent=None):
-        self._offsets = np.ascontiguousarray(offsets, np.int32)
-        if self._offsets.ndim != 1 or self._offsets.size < 2:
+        given = np.asarray(offsets)
+        if given.ndim != 1 or given.size < 2:
             raise ValueError("offsets: one entry per sequence and one behind the last")
+        if given.dtype.kind not in "iu" or int(given.min()) < -(1 << 31) or int(given.max()) >= 1 << 31:
+            raise ValueError("offsets: whole numbers of 32 bits")
+        self._offsets = np.ascontiguousarray(given, np.int32)
         self.c = ffi.GdnBatch(self._offsets.size - 1, self._offsets.ctypes.data_as(C.POINTER(C.c_int32)), base, parent)
         self._ref = C.byref(self.c)
         self.rows = int(self._offsets[-1])
