@@ -145,10 +145,10 @@ def test_one_ring_stands_for_both():
 def test_offsets_are_whole_numbers_that_fit():
     """What int32 cannot hold is refused, not taken for another row."""
     layer = ts.GatedDelta(2, 4, 64, 32, 4, ts.BF16)
-    for good in ([0, 3, 3], (0, 5), np.array([0, 7], np.int64), np.array([0, 7], np.uint8)):
+    for good in ([0, 3, 3], (0, 5), np.array([0, 7], np.int64), np.array([0, 7], np.uint8), np.array([0.0, 3.0])):
         b = layer.batch(good, P)
         assert [b.c.offsets[i] for i in range(len(good))] == list(good) and b.rows == good[-1]
-    for bad in (np.array([0, (1 << 32) + 3]), np.array([0, 1 << 31]), [0, 1 << 40], [0.0, 2.5], np.array([0, 3], np.float32), [0, True, None], np.array([[0, 3]]),
+    for bad in (np.array([0, (1 << 32) + 3]), np.array([0, 1 << 31]), [0, 1 << 40], [0.0, 2.5], [0.0, float("nan")], [0.0, float("inf")], [0, True, None], np.array([[0, 3]]),
                 np.array([0, (1 << 64) - 1], np.uint64), [], 3):
         with pytest.raises(ValueError):
             layer.batch(bad, P)

@@ -18,7 +18,7 @@ class Batch:
         given = np.asarray(offsets)
         if given.ndim != 1 or given.size < 2:
             raise ValueError("offsets: one entry per sequence and one behind the last")
-        if given.dtype.kind not in "iu" or int(given.min()) < -(1 << 31) or int(given.max()) >= 1 << 31:
+        if given.dtype.kind not in "iuf" or not all(-(1 << 31) <= x < 1 << 31 and x == int(x) for x in given.tolist()):
             raise ValueError("offsets: whole numbers of 32 bits")
         self._offsets = np.ascontiguousarray(given, np.int32)
         self.c = ffi.GdnBatch(self._offsets.size - 1, self._offsets.ctypes.data_as(C.POINTER(C.c_int32)), base, parent)
