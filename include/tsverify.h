@@ -512,7 +512,7 @@ int32_t tsv_gdn_conv(void* stream, const tsv_gdn_layer* layer, const tsv_gdn_bat
 /* The delta rule over prompts of any length, in blocks of 64 rows: state_out becomes the state behind each sequence's last row.
  * q, k: n_k_heads x k_dim a row, of unit length or shorter (the blocks' solution is built on that); v: n_v_heads x v_dim; g (a
  * value above 0 counts as 0) and beta as tsv_gdn_conv leaves them.  out: n_v_heads x v_dim a row; z NULL: o as it is.  The norm is
- * taken of o as rounded to the rows' type.  The workspace (device, 16-byte aligned) belongs to the call until it has run: calls
+ * taken of o in f32, as in tsv_gdn_step.  The workspace (device, 16-byte aligned) belongs to the call until it has run: calls
  * that may overlap in time take one each. */
 typedef struct {
     const void *q, *k, *v;

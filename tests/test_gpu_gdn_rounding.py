@@ -1,0 +1,77 @@
+"""What the prompts' rule (tsv_gdn_prefill) loses beside the one rounding of its results.
+
+A result rounded once lies within half a step of the rows' type of what was rounded; how much further from the 64-bit recurrence it lies
+(`excess`) is at most what the value was off before.  Of what a product of two-term operands adds at most 3 * 2^-18 is lost (2^-18 of
+either operand and of the product of the two lower terms); three products one behind the other (k S, T r, P u) make 9 * 2^-18, and in the
+2-norm, where these are of all signs, half of that: 2^-15 of a row's o at the most.  Under a gate y = o / r * w: o and the root r of its
+mean square both, 2^-14; f32 sums and exponentials stay below 2^-17.  2^-13 is allowed, an eighth of what fp16 rows lose to a rounding of o
+before the norm at the worst, 2^-11."""
+import numpy as np
+import pytest
+
+import turbospark_amd as ts
+from tests.gdn_common import Dev, Layer, from_bits, strided, to_bits
+from tests.test_gpu_gdn import Prompt
+
+pytestmark = pytest.mark.gpu
+BF, HF = ts.BF16, ts.F16
+
+
+def excess(got, want, dtype):
+    """How far got lies from want beyond half a step of the rows' type."""
+    bits, least = (11, -14) if dtype == HF else (8, -126)
+    size = np.maximum(np.maximum(np.abs(got), np.abs(want)), 2.0 ** least)
+    half = 2.0 ** (np.floor(np.log2(size)) - bits)
+    return np.maximum(np.abs(got - want) - half, 0.0)
+
+
+def sized(p, size):
+    """The prompt's values and state, `size` times as large."""
+    p.v = to_bits(from_bits(p.v, p.ly.dtype) * size, p.ly.dtype)
+    p.state = (p.state * size).astype(np.float32)
+    p.dv_.put(strided(p.v, p.io.v_stride))
+    given = p.state.copy()
+    for s in range(p.n):
+        if p.base[s] == 0:
+            given[s] = np.nan
+    p.din.put(given)
+
+
+def rows_of(p):
+    p.ly.gpu.prefill(p.batch, p.io)
+    width = p.ly.hv * p.ly.dv
+    return from_bits(p.out.get()[:p.T, :width], p.ly.dtype), p.want()[0]
+
+
+@pytest.mark.parametrize("hk,hv,dk,dv,lengths,size,scale", [
+    (2, 4, 64, 64, [130, 65], 1.0, 0.0),
+    (1, 2, 128, 48, [200], 4000.0, 64.0),         # o far above 65504
+    (1, 2, 128, 48, [200], 2.0 ** -13, 0.0),      # o of fp16's subnormal numbers
+    (2, 4, 64, 32, [2100], 4000.0, 64.0),         # in segments
+    (4, 8, 128, 128, [70] * 8, 2.0 ** -13, 0.0),  # two column tiles a workgroup
+    (1, 1, 256, 256, [70], 4000.0, 64.0),
+])
+def test_the_norm_takes_o_as_it_is(hk, hv, dk, dv, lengths, size, scale):
+    rng = np.random.default_rng(dk + dv)
+    p = Prompt(rng, Layer(rng, hk, hv, dk, dv, 4, HF, scale=scale), lengths, [s for s in range(len(lengths))], gated=True, pad=8)
+    sized(p, size)
+    rows, want = rows_of(p)
+    assert np.isfinite(rows).all()
+    off = excess(rows, want, HF)
+    assert np.linalg.norm(off) <= 2.0 ** -13 * np.linalg.norm(want), np.linalg.norm(off) / np.linalg.norm(want)
+
+
+def test_a_layer_without_norm_weights_needs_no_room_for_the_norm():
+    rng = np.random.default_rng(1)
+    ly = Layer(rng, 1, 2, 64, 32, 4, BF)
+    p = Prompt(rng, ly, [200], [3], gated=False)
+    bare = ts.GatedDelta(1, 2, 64, 32, 4, BF)
+    room = bare.prefill_workspace(p.batch)
+    assert room == ly.gpu.prefill_workspace(p.batch) - 4 * 64 * 2 * 32 * 4
+    ly.gpu.prefill(p.batch, p.io)
+    rows, S = p.check()
+    p.ws = Dev(np.full(room // 4 + 4, 7.0, np.float32))
+    p.io.workspace, p.io.workspace_bytes = p.ws.ptr, room
+    p.out.put(np.full_like(p.out.a, 0x1234))
+    bare.prefill(p.batch, p.io)
+    assert np.array_equal(p.out.get(), rows) and np.array_equal(p.dout.get(), S) and (p.ws.get()[room // 4:] == 7).all()

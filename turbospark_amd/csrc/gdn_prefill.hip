@@ -10,8 +10,9 @@
 // v - e^G kS are two bf16 terms each (2^-18, split2: 5e-6 of the state's norm after thousands of rows; one term would leave 2e-3), k and
 // q the rows' own bits (fp16 rows: two terms, exact).  P u, which ends in a rounding to the rows' type, is one term by one for bf16 rows
 // (2.5e-3 of the result's norm with that rounding's 1.7e-3 in it; two by two costs the walk 15%) and two by two for fp16.  T's inverse is
-// f32 throughout, the running sum of g 64 bits, since differences of a long sum are what the decays are made of.  o is rounded to the
-// rows' type before the gated norm reads it again: half a step more in the result, where f32 would move twice the bytes.
+// f32 throughout, the running sum of g 64 bits, since differences of a long sum are what the decays are made of.  The gated norm reads o
+// in f32 from the workspace: rounded to the rows' type before, fp16 rows had no o above 65504 and no bits in a small one, and the result
+// of bf16 rows was half a step further off.
 #include "gdn.h"
 
 #include <algorithm>
@@ -33,6 +34,7 @@ struct PrefillArgs {
     float* gates;    // ... and e^G, e^{G_end - G}
     float* ends;     // ... and per (segment, value head) what a segment does to a state: [v_dim][k_dim] from nothing, then [k_dim][k_dim]
     float* starts;   // ... and the states that sequences of several segments start from: state_out may be state_in
+    float* o32;      // ... and the rows of o that the gated norm reads
     int32_t tiles;   // column tiles of a head in the walk
     int32_t split;   // the blocks' matrices: a workgroup per value head
     int32_t seg_blocks;  // blocks of a segment, the last of a sequence may have fewer
@@ -330,8 +332,8 @@ struct Walk {
     static constexpr int TR = F16 ? 2 : 1, KS = DK / 32, SD = DK / 64;
     // LDS, all in operand order [k step][nt][term][lane]
     static constexpr int S_AT = 0, R_AT = KS * NT * 2 * 64, U_AT = R_AT + 2 * NT * 2 * 64, D_AT = U_AT + 2 * NT * TR * 64;
-    // v as [column][VS], the decays e^G and e^{G_end - G}, and the output rows on their way out, a region per wave
-    static constexpr int V_AT = D_AT + 2 * NT * 2 * 64, VS = 72, G_AT = V_AT + 16 * NT * VS / 8, O_AT = G_AT + 32, LDS = O_AT + 64 * 16 * NT / 8;
+    // v as [column][VS], the decays e^G and e^{G_end - G}, and the output rows on their way out, a region per wave (f32 rows of OS values)
+    static constexpr int V_AT = D_AT + 2 * NT * 2 * 64, VS = 72, G_AT = V_AT + 16 * NT * VS / 8, O_AT = G_AT + 32, OS = 16 * NT + 4, LDS = O_AT + 64 * OS / 4;
     uint4* lds;
     int lane, w, l16, gq;
 
@@ -356,9 +358,13 @@ struct Walk {
     }
 };
 
-template <int DK, bool F16, int NT, bool ENDS>
+// What a walk is for: o in the rows' type, o in f32 for the norm behind it, or what the segments do to a state.
+enum WalkFor { ROWS, NORM, SEGMENTS };
+
+template <int DK, bool F16, int NT, WalkFor FOR>
 __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape sh, GdnBatch bt, PrefillArgs p) {
     typedef Walk<DK, F16, NT> W;
+    constexpr bool ENDS = FOR == SEGMENTS;
     constexpr int TR = W::TR, KS = W::KS, SD = W::SD;
     extern __shared__ uint4 lds[];
     const int tid = threadIdx.x, lane = tid & 63, w8 = __builtin_amdgcn_readfirstlane(tid >> 6), w = w8 & 3, l16 = lane & 15, gq = lane >> 4;
@@ -440,11 +446,14 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         typedef uint32_t piece __attribute__((ext_vector_type(2 * NT)));
         const int prow = 16 * w + (lane >> 2), pcol = (lane & 3) * 4 * NT;
         const uint16_t* vp = p.v + (int64_t)first * p.v_stride + h * sh.dv + (unit ? 0 : tile * 16 * NT) + pcol;
-        char* op = (char*)(p.out + (int64_t)first * p.out_stride + h * sh.dv + tile * 16 * NT);
-        const int64_t o_step = p.out_stride * (2 * BLK);
-        const uint32_t o_off = prow * (uint32_t)(2 * p.out_stride) + 2 * pcol;
+        constexpr int OB = FOR == NORM ? 4 : 2;  // bytes of a value of o
+        const int64_t o_stride = FOR == NORM ? sh.hv * sh.dv : p.out_stride;
+        char* op = (FOR == NORM ? (char*)p.o32 : (char*)p.out) + OB * ((int64_t)first * o_stride + h * sh.dv + tile * 16 * NT);
+        const int64_t o_step = o_stride * (OB * BLK);
+        const uint32_t o_off = prow * (uint32_t)(OB * o_stride) + OB * pcol;
         uint16_t* vt = (uint16_t*)(lds + W::V_AT);
         uint16_t* ot = (uint16_t*)(lds + W::O_AT) + w * 16 * 16 * NT;
+        float* of = (float*)(lds + W::O_AT) + w * 16 * W::OS;
         piece vr;
         float2 gr;
         auto ask_v = [&](int b) {  // (rows behind the sequence's last are taken from it: T is 0 there)
@@ -536,13 +545,22 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
 #pragma unroll
             for (int t = 0; t < NT; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) ot[(4 * gq + r) * 16 * NT + 16 * t + l16] = row_bits<F16>(sh.scale * o[t][r]);
+                for (int r = 0; r < 4; r++) {
+                    if constexpr (FOR == NORM) of[(4 * gq + r) * W::OS + 16 * t + l16] = sh.scale * o[t][r];
+                    else ot[(4 * gq + r) * 16 * NT + 16 * t + l16] = row_bits<F16>(sh.scale * o[t][r]);
+                }
             wave_lds_fence();
-            const piece out = *(const piece*)(ot + (lane >> 2) * 16 * NT + pcol);
             // (a buffer's end at the sequence's last row: stores behind it are dropped by the hardware, without a branch)
-            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(op, 0, ((uint32_t)min(rows - b * BLK, BLK) - 1) * (uint32_t)(2 * p.out_stride) + 32 * NT, 0x00027000);
-            if constexpr (NT == 1) __builtin_amdgcn_raw_buffer_store_b64(out, rsrc, o_off, 0, 0);
-            else __builtin_amdgcn_raw_buffer_store_b128(out, rsrc, o_off, 0, 0);
+            const auto rsrc = __builtin_amdgcn_make_buffer_rsrc(op, 0, ((uint32_t)min(rows - b * BLK, BLK) - 1) * (uint32_t)(OB * o_stride) + 16 * OB * NT, 0x00027000);
+            if constexpr (FOR == NORM) {
+                typedef uint32_t four __attribute__((ext_vector_type(4)));
+#pragma unroll
+                for (int t = 0; t < NT; t++) __builtin_amdgcn_raw_buffer_store_b128(*(const four*)(of + (lane >> 2) * W::OS + pcol + 4 * t), rsrc, o_off, 16 * t, 0);
+            } else {
+                const piece out = *(const piece*)(ot + (lane >> 2) * 16 * NT + pcol);
+                if constexpr (NT == 1) __builtin_amdgcn_raw_buffer_store_b64(out, rsrc, o_off, 0, 0);
+                else __builtin_amdgcn_raw_buffer_store_b128(out, rsrc, o_off, 0, 0);
+            }
             op += o_step;
         }
         return;
@@ -763,17 +781,18 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
 #undef GDN_FENCE
 #undef GDN_ARRIVED
 
-// ---- the gated norm, in place --------------------------------------------------------------------------------------------------------
-// v_dim / 8 of GROUP neighbouring lanes hold a head's row.  Bound by memory: 8192 rows of 32 heads of 128, 201 MB, 35 us (5.7 TB/s).
+// ---- the gated norm ----------------------------------------------------------------------------------------------------------------------
+// v_dim / 8 of GROUP neighbouring lanes hold a head's row.  Bound by memory: 8192 rows of 32 heads of 128, 268 MB, NORM_US us.
 template <bool F16>
-__global__ __launch_bounds__(256) void k_gdn_norm(GdnShape sh, uint16_t* out, int64_t out_stride, const uint16_t* z, int64_t z_stride, uint32_t heads, int group) {
+__global__ __launch_bounds__(256) void k_gdn_norm(GdnShape sh, const float* o, uint16_t* out, int64_t out_stride, const uint16_t* z, int64_t z_stride, uint32_t heads, int group) {
     const uint32_t at = (blockIdx.x * 256 + threadIdx.x) / group, row = at / sh.hv, h = at - row * sh.hv;
     const int c = (threadIdx.x & (group - 1)) * 8;
     const bool in = at < heads && c < sh.dv;
-    uint16_t* o = out + (int64_t)row * out_stride + h * sh.dv + c;
     float x[8] = {}, y[8] = {}, sum = 0.0f;
     if (in) {
-        row8_f32<F16>(*(const uint4*)o, x);
+        const float4* from = (const float4*)(o + (int64_t)at * sh.dv + c);
+        const float4 a = from[0], b = from[1];
+        x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
         row8_f32<F16>(*(const uint4*)(z + (int64_t)row * z_stride + h * sh.dv + c), y);
     }
 #pragma unroll
@@ -783,7 +802,7 @@ __global__ __launch_bounds__(256) void k_gdn_norm(GdnShape sh, uint16_t* out, in
     const float f = rsqrtf(sum / (float)sh.dv + sh.norm_eps);
 #pragma unroll
     for (int e = 0; e < 8; e++) x[e] = x[e] * f * sh.norm[c + e] * silu_f32(y[e]);
-    *(uint4*)o = make_uint4(row_pair<F16>(x[0], x[1]), row_pair<F16>(x[2], x[3]), row_pair<F16>(x[4], x[5]), row_pair<F16>(x[6], x[7]));
+    *(uint4*)(out + (int64_t)row * out_stride + h * sh.dv + c) = make_uint4(row_pair<F16>(x[0], x[1]), row_pair<F16>(x[2], x[3]), row_pair<F16>(x[4], x[5]), row_pair<F16>(x[6], x[7]));
 }
 
 namespace {
@@ -804,7 +823,7 @@ int segment_blocks(const GdnShape& sh, const GdnBatch& bt) {
 }
 
 struct Sizes {
-    int64_t kt, tp, gates, ends, starts, total;  // bytes
+    int64_t kt, tp, gates, ends, starts, o32, total;  // bytes
     int64_t blocks, segments;
     int seg_blocks;
 };
@@ -823,7 +842,8 @@ Sizes workspace_of(const GdnShape& sh, const GdnBatch& bt, int dk, bool f16) {
     z.gates = z.blocks * sh.hv * 512;
     z.ends = z.seg_blocks == INT32_MAX ? 0 : z.segments * sh.hv * (sh.dv + dk) * dk * 4;
     z.starts = z.seg_blocks == INT32_MAX ? 0 : (int64_t)bt.n_seq * sh.hv * sh.dv * dk * 4;
-    z.total = z.kt + z.tp + z.gates + z.ends + z.starts;
+    z.o32 = sh.norm ? z.blocks * BLK * sh.hv * sh.dv * 4 : 0;  // (without norm weights a layer has no gated norm)
+    z.total = z.kt + z.tp + z.gates + z.ends + z.starts + z.o32;
     return z;
 }
 
@@ -840,17 +860,27 @@ int launch_blocks(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, Prefil
     return TSV_OK;
 }
 
-template <int DK, bool F16, int NT, bool ENDS>
+template <int DK, bool F16, int NT, WalkFor FOR>
 int launch_walk(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, PrefillArgs& p) {
     const size_t lds = (size_t)Walk<DK, F16, NT>::LDS * 16;
     static OncePerDevice once;
-    const int rc = allow_lds((const void*)k_gdn_walk<DK, F16, NT, ENDS>, lds, once);
+    const int rc = allow_lds((const void*)k_gdn_walk<DK, F16, NT, FOR>, lds, once);
     if (rc) return rc;
-    p.tiles = (sh.dv + (ENDS ? DK : 0)) / (16 * NT);
+    p.tiles = (sh.dv + (FOR == SEGMENTS ? DK : 0)) / (16 * NT);
     const int heads = p.seg_of[bt.n_seq] * sh.hk;
-    hipLaunchKernelGGL((k_gdn_walk<DK, F16, NT, ENDS>), dim3((heads + 7) / 8 * 8 * sh.rep * p.tiles), dim3(walk_threads<DK, NT>), lds, st, sh, bt, p);
+    hipLaunchKernelGGL((k_gdn_walk<DK, F16, NT, FOR>), dim3((heads + 7) / 8 * 8 * sh.rep * p.tiles), dim3(walk_threads<DK, NT>), lds, st, sh, bt, p);
     TSV_HIP(hipGetLastError());
     return TSV_OK;
+}
+
+template <int DK, bool F16, WalkFor FOR>
+int launch_rows(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, PrefillArgs& p) {
+    // Two column tiles a workgroup where that still gives every compute unit one: they share what a block reads (6 sequences, 32 heads of
+    // 128: 72 us against 106); else one, for the shorter way through a block (8192 rows, 32 heads: 185 us against 208).  k_dim 256 has no
+    // registers for two.
+    if constexpr (DK < 256)
+        if (sh.dv % 32 == 0 && (int64_t)p.seg_of[bt.n_seq] * sh.hv * (sh.dv / 32) >= 256) return launch_walk<DK, F16, 2, FOR>(st, sh, bt, p);
+    return launch_walk<DK, F16, 1, FOR>(st, sh, bt, p);
 }
 
 template <int DK, bool F16>
@@ -859,18 +889,13 @@ int launch_prefill(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, Prefi
         const int rc = launch_blocks<DK, F16>(st, sh, bt, p, blocks);
         if (rc) return rc;
     }
-    // Two column tiles a workgroup where that still gives every compute unit one: they share what a block reads (6 sequences, 32 heads of
-    // 128: 72 us against 106); else one, for the shorter way through a block (8192 rows, 32 heads: 185 us against 208).  k_dim 256 has no
-    // registers for two.
     if (p.seg_of[bt.n_seq] > bt.n_seq) {
         int rc;
-        if constexpr (DK < 256) rc = sh.dv % 32 == 0 ? launch_walk<DK, F16, 2, true>(st, sh, bt, p) : launch_walk<DK, F16, 1, true>(st, sh, bt, p);
-        else rc = launch_walk<DK, F16, 1, true>(st, sh, bt, p);
+        if constexpr (DK < 256) rc = sh.dv % 32 == 0 ? launch_walk<DK, F16, 2, SEGMENTS>(st, sh, bt, p) : launch_walk<DK, F16, 1, SEGMENTS>(st, sh, bt, p);
+        else rc = launch_walk<DK, F16, 1, SEGMENTS>(st, sh, bt, p);
         if (rc) return rc;
     }
-    if constexpr (DK < 256)
-        if (sh.dv % 32 == 0 && (int64_t)p.seg_of[bt.n_seq] * sh.hv * (sh.dv / 32) >= 256) return launch_walk<DK, F16, 2, false>(st, sh, bt, p);
-    return launch_walk<DK, F16, 1, false>(st, sh, bt, p);
+    return p.o32 ? launch_rows<DK, F16, NORM>(st, sh, bt, p) : launch_rows<DK, F16, ROWS>(st, sh, bt, p);
 }
 
 }  // namespace
@@ -925,6 +950,7 @@ extern "C" int32_t tsv_gdn_prefill(void* stream, const tsv_gdn_layer* layer, con
     p.gates = (float*)(ws + z.kt + z.tp);
     p.ends = (float*)(ws + z.kt + z.tp + z.gates);
     p.starts = (float*)(ws + z.kt + z.tp + z.gates + z.ends);
+    p.o32 = io->z ? (float*)(ws + z.kt + z.tp + z.gates + z.ends + z.starts) : nullptr;
     p.seg_blocks = z.seg_blocks;
     p.block_of[0] = p.seg_of[0] = 0;
     for (int s = 0; s < bt.n_seq; s++) {
@@ -942,10 +968,11 @@ extern "C" int32_t tsv_gdn_prefill(void* stream, const tsv_gdn_layer* layer, con
     const int rows = bt.off[bt.n_seq], at_once = (1 << 26) / sh.hv;  // (a launch has 2^32 threads at most)
     for (int r = 0; r < rows; r += at_once) {
         const uint32_t heads = (uint32_t)std::min(at_once, rows - r) * sh.hv, wgs = (uint32_t)(((uint64_t)heads * group + 255) / 256);
+        const float* o = p.o32 + (int64_t)r * sh.hv * sh.dv;
         uint16_t* out = p.out + (int64_t)r * p.out_stride;
         const uint16_t* gate = (const uint16_t*)io->z + (int64_t)r * io->z_stride;
-        if (f16) hipLaunchKernelGGL((k_gdn_norm<true>), dim3(wgs), dim3(256), 0, st, sh, out, p.out_stride, gate, io->z_stride, heads, group);
-        else hipLaunchKernelGGL((k_gdn_norm<false>), dim3(wgs), dim3(256), 0, st, sh, out, p.out_stride, gate, io->z_stride, heads, group);
+        if (f16) hipLaunchKernelGGL((k_gdn_norm<true>), dim3(wgs), dim3(256), 0, st, sh, o, out, p.out_stride, gate, io->z_stride, heads, group);
+        else hipLaunchKernelGGL((k_gdn_norm<false>), dim3(wgs), dim3(256), 0, st, sh, o, out, p.out_stride, gate, io->z_stride, heads, group);
     }
     TSV_HIP(hipGetLastError());
     return TSV_OK;
