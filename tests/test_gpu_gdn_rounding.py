@@ -75,3 +75,21 @@ def test_a_layer_without_norm_weights_needs_no_room_for_the_norm():
     p.out.put(np.full_like(p.out.a, 0x1234))
     bare.prefill(p.batch, p.io)
     assert np.array_equal(p.out.get(), rows) and np.array_equal(p.dout.get(), S) and (p.ws.get()[room // 4:] == 7).all()
+
+
+@pytest.mark.parametrize("hk,hv,dk,dv,lengths,dtype", [
+    (2, 4, 64, 64, [130, 65], BF),
+    (1, 3, 128, 48, [200, 1, 64], BF),
+    (2, 4, 128, 128, [300], HF),
+    (1, 2, 64, 32, [2100], BF),                   # in segments
+    (4, 8, 128, 128, [70] * 8, BF),               # two column tiles a workgroup
+    (16, 80, 64, 16, [600], BF),                  # several value heads a workgroup
+    (1, 1, 256, 256, [70], BF),
+])
+@pytest.mark.parametrize("gated", [True, False])
+def test_rows_are_rounded_once(hk, hv, dk, dv, lengths, dtype, gated):
+    rng = np.random.default_rng(dk + dv + 1)
+    p = Prompt(rng, Layer(rng, hk, hv, dk, dv, 4, dtype), lengths, [s for s in range(len(lengths))], gated=gated, pad=8)
+    rows, want = rows_of(p)
+    off = excess(rows, want, dtype)
+    assert np.linalg.norm(off) <= 2.0 ** -13 * np.linalg.norm(want), np.linalg.norm(off) / np.linalg.norm(want)

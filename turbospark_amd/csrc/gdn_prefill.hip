@@ -8,9 +8,8 @@
 //
 // Precision: the state is f32 and never rounded; as operands of the bf16 matrix instruction the state, T, u and the difference
 // v - e^G kS are two bf16 terms each (2^-18, split2: 5e-6 of the state's norm after thousands of rows; one term would leave 2e-3), k and
-// q the rows' own bits (fp16 rows: two terms, exact).  P u, which ends in a rounding to the rows' type, is one term by one for bf16 rows
-// (2.5e-3 of the result's norm with that rounding's 1.7e-3 in it; two by two costs the walk 15%) and two by two for fp16.  T's inverse is
-// f32 throughout, the running sum of g 64 bits, since differences of a long sum are what the decays are made of.  The gated norm reads o
+// q the rows' own bits (fp16 rows: two terms, exact).  P and u are two terms each in P u (one by one left bf16 rows 2.6e-3 off, where their
+// rounding makes 1.7e-3).  T's inverse is f32 throughout, the running sum of g 64 bits, since differences of a long sum are what the decays are made of.  The gated norm reads o
 // in f32 from the workspace: rounded to the rows' type before, fp16 rows had no o above 65504 and no bits in a small one, and the result
 // of bf16 rows was half a step further off.
 #include "gdn.h"
@@ -91,10 +90,12 @@ __device__ __forceinline__ int sequence_of(const int32_t* starts, int n, int at)
 // contraction takes rows 4 gq + r in step r.  8192 rows, 16 key and 32 value heads of 128: 76 us for 43 MB read and 174 MB written
 // (2.9 TB/s); the waits of one workgroup, three on a compute unit, bound it.  Few blocks have a workgroup per value head instead
 // (split), each making the products again: 65 rows, 8 heads over 4, 14.4 us against 10.1.
-constexpr int PS = 72;  // row stride (2-byte values) of P in LDS
+// Where P's value (i, j) lies in LDS: rows of 64 values, whose eight 16-byte units take turns from row to row (a column of them, as the
+// fragments are read, would else lie in two banks)
+__device__ __forceinline__ int p_at(int i, int j) { return i * BLK + (((j >> 3) ^ (i & 7)) << 3) + (j & 7); }
 // 16-byte units of LDS that hold k's operands, then P
 template <int DK, int TR>
-constexpr int blocks_operands = KFRAGS<DK, TR> * 64 > TR * BLK * PS / 8 ? KFRAGS<DK, TR> * 64 : TR * BLK * PS / 8;
+constexpr int blocks_operands = KFRAGS<DK, TR> * 64 > 2 * BLK * BLK / 8 ? KFRAGS<DK, TR> * 64 : 2 * BLK * BLK / 8;
 
 // What a head's decays are in a block.  e^{G_i - G_j} of rows in different row tiles is made of three factors of at most 1: from j to its
 // tile's end, the tiles between, and from the start of i's tile to i; inside a tile it is one exponential of a 64-bit difference.
@@ -110,7 +111,7 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
     constexpr int TR = F16 ? 2 : 1, KS = DK / 32;
     extern __shared__ uint4 lds[];
     uint4* kf = lds;                                   // [row tile][k step][term][lane]
-    uint16_t* P = (uint16_t*)lds;                      // [term][64][PS], where the operands were
+    uint16_t* P = (uint16_t*)lds;                      // [term][64][64], where the operands were
     float* A = (float*)(lds + blocks_operands<DK, TR>);  // [64][MS]
     float* T = A + BLK * MS;
     BlockGates* gates = (BlockGates*)(T + BLK * MS);   // of GATE_HEADS heads
@@ -214,8 +215,8 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
             auto put_p = [&](int i, int j, float x) {
                 __bf16 hi, lo;
                 split2(x, hi, lo);
-                P[i * PS + j] = __builtin_bit_cast(uint16_t, hi);
-                if constexpr (TR == 2) P[(BLK + i) * PS + j] = __builtin_bit_cast(uint16_t, lo);
+                P[p_at(i, j)] = __builtin_bit_cast(uint16_t, hi);
+                P[BLK * BLK + p_at(i, j)] = __builtin_bit_cast(uint16_t, lo);
             };
 #pragma unroll
             for (int c = 0; c < 3; c++) {
@@ -280,7 +281,7 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
             }
         }
         __syncthreads();
-        uint4* to = p.tp + ((int64_t)blk * sh.hv + h) * (TFRAGS * (2 + TR) * 64);
+        uint4* to = p.tp + ((int64_t)blk * sh.hv + h) * (TFRAGS * 4 * 64);
 #pragma unroll
         for (int ks = 0; ks < 2; ks++) {
             if (ks > w / 2) continue;
@@ -297,7 +298,7 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
             to[(2 * f + 1) * 64 + lane] = tl;
             const bool zero = 32 * ks + 8 * gq >= 16 * (w + 1);  // (columns of row tiles behind this one)
 #pragma unroll
-            for (int e = 0; e < TR; e++) to[(2 * TFRAGS + TR * f + e) * 64 + lane] = zero ? make_uint4(0, 0, 0, 0) : *(const uint4*)(P + (e * BLK + row) * PS + j0);
+            for (int e = 0; e < 2; e++) to[(2 * TFRAGS + 2 * f + e) * 64 + lane] = zero ? make_uint4(0, 0, 0, 0) : *(const uint4*)(P + e * BLK * BLK + p_at(row, j0));
         }
         __syncthreads();
     }
@@ -331,7 +332,7 @@ template <int DK, bool F16, int NT>
 struct Walk {
     static constexpr int TR = F16 ? 2 : 1, KS = DK / 32, SD = DK / 64;
     // LDS, all in operand order [k step][nt][term][lane]
-    static constexpr int S_AT = 0, R_AT = KS * NT * 2 * 64, U_AT = R_AT + 2 * NT * 2 * 64, D_AT = U_AT + 2 * NT * TR * 64;
+    static constexpr int S_AT = 0, R_AT = KS * NT * 2 * 64, U_AT = R_AT + 2 * NT * 2 * 64, D_AT = U_AT + 2 * NT * 2 * 64;
     // v as [column][VS], the decays e^G and e^{G_end - G}, and the output rows on their way out, a region per wave (f32 rows of OS values)
     static constexpr int V_AT = D_AT + 2 * NT * 2 * 64, VS = 72, G_AT = V_AT + 16 * NT * VS / 8, O_AT = G_AT + 32, OS = 16 * NT + 4, LDS = O_AT + 64 * OS / 4;
     uint4* lds;
@@ -385,9 +386,9 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
     const float* ends = p.ends + ((int64_t)p.seg_of[s] * sh.hv + h) * (sh.dv + DK) * DK;  // of the sequence's first segment
     const int64_t ends_step = (int64_t)sh.hv * (sh.dv + DK) * DK;
     // uniform addresses of the block asked for, and what a lane adds to them (in bytes)
-    const char* tpp = (const char*)(p.tp + (b0 * sh.hv + h) * (TFRAGS * (2 + TR) * 64));
+    const char* tpp = (const char*)(p.tp + (b0 * sh.hv + h) * (TFRAGS * 4 * 64));
     const char* gp = (const char*)(p.gates + (b0 * sh.hv + h) * 128);
-    const int64_t tp_step = (int64_t)sh.hv * (TFRAGS * (2 + TR) * 1024), g_step = (int64_t)sh.hv * 512;
+    const int64_t tp_step = (int64_t)sh.hv * (TFRAGS * 4 * 1024), g_step = (int64_t)sh.hv * 512;
     const uint32_t lane16 = lane * 16;
     // (waves of rows 0 and 16 have one fragment of T and P where the others have two: they ask for theirs twice and clear the copy, so
     // that every wave has the same loads under way and a wait is for the ones it needs)
@@ -398,7 +399,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         return __builtin_bit_cast(bf16x8, make_uint4(f.x & second, f.y & second, f.z & second, f.w & second));
     };
     if (walk_threads<DK, NT> > 512 && w8 == 8) {  // ---- the wave that brings what is four blocks ahead into the XCD's L2, this workgroup's share of it
-        constexpr int AHEAD = 4, LINES = 3 * KFRAGS<DK, TR> * 8 + TFRAGS * (2 + TR) * 8, SHARE = 3;
+        constexpr int AHEAD = 4, LINES = 3 * KFRAGS<DK, TR> * 8 + TFRAGS * 4 * 8, SHARE = 3;
         const char* kreg = (const char*)(p.kt + (b0 * sh.hk + hk) * (3 * KFRAGS<DK, TR> * 64));
         const int64_t k_step = (int64_t)sh.hk * (3 * KFRAGS<DK, TR> * 1024);
         const char* vreg = (const char*)(p.v + (int64_t)first * p.v_stride + h * sh.dv + (unit ? 0 : tile * 16 * NT));
@@ -428,7 +429,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
     if (w8 >= 4) {  // ---- the output's waves
         const char* qp = (const char*)(p.kt + ((b0 * sh.hk + hk) * 3 + 1) * (KFRAGS<DK, TR> * 64) + w * KS * TR * 64);
         const int64_t q_step = (int64_t)sh.hk * (3 * KFRAGS<DK, TR> * 1024);
-        uint4 qr[KS][TR], pr[2][TR];
+        uint4 qr[KS][TR], pr[2][2];
         auto ask_q = [&]() {
 #pragma unroll
             for (int t = 0; t < KS; t++)
@@ -437,9 +438,9 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         };
         auto ask_p = [&]() {
 #pragma unroll
-            for (int e = 0; e < TR; e++) {
-                pr[0][e] = *(const uint4*)(tpp + (2 * TFRAGS + TR * f0 + e) * 1024 + lane16);
-                pr[1][e] = *(const uint4*)(tpp + (2 * TFRAGS + TR * f1 + e) * 1024 + lane16);
+            for (int e = 0; e < 2; e++) {
+                pr[0][e] = *(const uint4*)(tpp + (2 * TFRAGS + 2 * f0 + e) * 1024 + lane16);
+                pr[1][e] = *(const uint4*)(tpp + (2 * TFRAGS + 2 * f1 + e) * 1024 + lane16);
             }
         };
         // a lane's piece of the rows: a quarter of row lane / 4 of the wave's sixteen
@@ -524,22 +525,29 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
             __syncthreads();
             ask_q();
             __syncthreads();
-            bf16x8 u[2][NT][TR];
+            bf16x8 u[2][NT][2];
 #pragma unroll
             for (int ks = 0; ks < 2; ks++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) x.template get<TR>(W::U_AT, ks, t, u[ks][t]);
+                for (int t = 0; t < NT; t++) x.template get<2>(W::U_AT, ks, t, u[ks][t]);
             put_v();  // (the others are done with this block's)
             GDN_FENCE;
             ask_v(b + 2);
+            gf4 o3[NT];
+#pragma unroll
+            for (int t = 0; t < NT; t++) o2[t] = o3[t] = gf4{0, 0, 0, 0};
 #pragma unroll
             for (int ks = 0; ks < 2; ks++) {
-                bf16x8 a[TR];
+                const bf16x8 a0 = fragment(pr[ks][0], ks), a1 = fragment(pr[ks][1], ks);
 #pragma unroll
-                for (int e = 0; e < TR; e++) a[e] = fragment(pr[ks][e], ks);
-#pragma unroll
-                for (int t = 0; t < NT; t++) o[t] = mfma_terms<TR, TR>(a, u[ks][t], o[t]);
+                for (int t = 0; t < NT; t++) {
+                    o[t] = mfma_bf16(a0, u[ks][t][0], o[t]);
+                    o2[t] = mfma_bf16(a0, u[ks][t][1], o2[t]);
+                    o3[t] = mfma_bf16(a1, u[ks][t][0], o3[t]);
+                }
             }
+#pragma unroll
+            for (int t = 0; t < NT; t++) o[t] += o2[t] + o3[t];
             GDN_FENCE;
             ask_p();
 #pragma unroll
@@ -726,7 +734,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
             for (int t = 0; t < NT; t++) {
                 u[t] += u2[t];
                 x.template put<2>(W::D_AT, w >> 1, t, 2 * (w & 1) + (gq >> 1), ed * u[t]);
-                if constexpr (!ENDS) x.template put<TR>(W::U_AT, w >> 1, t, 2 * (w & 1) + (gq >> 1), u[t]);
+                if constexpr (!ENDS) x.template put<2>(W::U_AT, w >> 1, t, 2 * (w & 1) + (gq >> 1), u[t]);
             }
 #pragma unroll
             for (int i = 0; i < SD; i++)
@@ -838,7 +846,7 @@ Sizes workspace_of(const GdnShape& sh, const GdnBatch& bt, int dk, bool f16) {
         z.segments += std::max<int64_t>(1, (blocks_of(bt, s) + z.seg_blocks - 1) / z.seg_blocks);
     }
     z.kt = z.blocks * sh.hk * (3 * (dk / 8) * tr * 1024);
-    z.tp = z.blocks * sh.hv * (TFRAGS * (2 + tr) * 1024);
+    z.tp = z.blocks * sh.hv * (TFRAGS * 4 * 1024);
     z.gates = z.blocks * sh.hv * 512;
     z.ends = z.seg_blocks == INT32_MAX ? 0 : z.segments * sh.hv * (sh.dv + dk) * dk * 4;
     z.starts = z.seg_blocks == INT32_MAX ? 0 : (int64_t)bt.n_seq * sh.hv * sh.dv * dk * 4;
