@@ -93,3 +93,33 @@ def test_rows_are_rounded_once(hk, hv, dk, dv, lengths, dtype, gated):
     rows, want = rows_of(p)
     off = excess(rows, want, dtype)
     assert np.linalg.norm(off) <= 2.0 ** -13 * np.linalg.norm(want), np.linalg.norm(off) / np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("hk,hv,dk,dv,lengths,dtype", [
+    (2, 4, 64, 64, [130, 65], BF),
+    (2, 4, 64, 64, [130, 65], HF),
+    (1, 3, 128, 48, [700, 1, 64], BF),
+    (1, 2, 128, 128, [300], HF),
+    (1, 2, 64, 32, [2100], BF),                   # in segments
+    (1, 1, 128, 48, [2111], HF),
+    (1, 1, 256, 32, [2200], BF),
+    (4, 8, 128, 128, [70] * 8, BF),               # two column tiles a workgroup
+    (16, 80, 64, 16, [600], HF),                  # several value heads a workgroup
+    (1, 1, 256, 256, [170], HF),
+])
+@pytest.mark.parametrize("decay", [0.1, 0.002])
+def test_states_are_those_of_32_bits(hk, hv, dk, dv, lengths, dtype, decay):
+    """What a block adds to the state in f32 is off by its sums of 64 to 256 products (2^-24 of what they have reached, of all signs: 16 *
+    2^-25 = 2^-21 in the 2-norm), three one behind the other, by the inverse and by the exponentials (2^-22 each): 2^-20 together.  Blocks
+    add up where nothing decays, but of all signs too, and the recurrence only contracts: 2^-19 is allowed.  Operands of two bf16 terms,
+    2^-18 each, do not keep to it."""
+    rng = np.random.default_rng(dk + dv + 2)
+    p = Prompt(rng, Layer(rng, hk, hv, dk, dv, 4, dtype), lengths, [s for s in range(len(lengths))], gated=False)
+    p.g = (-decay * rng.random(p.g.shape)).astype(np.float32)
+    p.dg.put(np.concatenate([p.g, np.full((1, hv), np.nan, np.float32)]))
+    p.ly.gpu.prefill(p.batch, p.io)
+    S, want = p.dout.get(), p.want()[1]
+    for s in range(p.n):
+        off = np.linalg.norm(S[s] - want[s]) / np.linalg.norm(want[s])
+        print("state off by 2^%.2f" % np.log2(off))
+        assert off <= 2.0 ** -19, (s, off)

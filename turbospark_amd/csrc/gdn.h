@@ -74,6 +74,12 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
     lo = row_pair<false>(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u));
 }
 
+// ... as three: what they leave out is 2^-27 of the value at most, less than f32 itself holds
+__device__ __forceinline__ void split3(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+    hi = row_pair<false>(x, y);
+    split2(x - __uint_as_float(hi << 16), y - __uint_as_float(hi & 0xFFFF0000u), mid, lo);
+}
+
 // a store that does not stay in the L2: it is on its way to memory while the kernel runs, not when it ends
 __device__ __forceinline__ void store_through(void* to, gf4 x) { __builtin_nontemporal_store(x, (gf4*)to); }
 

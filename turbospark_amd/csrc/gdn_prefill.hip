@@ -6,12 +6,13 @@
 // k_gdn_blocks makes T diag(beta), P, k transposed and the decays of every block at once, k_gdn_walk goes through the blocks of a
 // sequence with 16 NT columns of one head's state in registers, k_gdn_norm is the gated norm of the result.
 //
-// Precision: the state is f32 and never rounded; as operands of the bf16 matrix instruction the state, T, u and the difference
-// v - e^G kS are two bf16 terms each (2^-18, split2: 5e-6 of the state's norm after thousands of rows; one term would leave 2e-3), k and
-// q the rows' own bits (fp16 rows: two terms, exact).  P and u are two terms each in P u (one by one left bf16 rows 2.6e-3 off, where their
-// rounding makes 1.7e-3).  T's inverse is f32 throughout, the running sum of g 64 bits, since differences of a long sum are what the decays are made of.  The gated norm reads o
-// in f32 from the workspace: rounded to the rows' type before, fp16 rows had no o above 65504 and no bits in a small one, and the result
-// of bf16 rows was half a step further off.
+// Precision: the state is f32 and never rounded.  In what makes it, k S and k^T u, it and u are three bf16 terms each (2^-27, split3), k the
+// rows' own bits (fp16 rows: two terms, exact); T (v - e^G kS) is made by the f32 instruction from f32 operands.  The state is then as far
+// off as one of plain 32-bit sums, 2e-7 to 1e-6 of its norm after thousands of rows (two terms throughout: 5e-6; one would leave 2e-3).
+// What only goes to the output, q S and P u, has two terms by two (2^-18, split2), so that the rows' own rounding is what a result is off by
+// (P u one term by one left bf16 rows 2.6e-3 off for their rounding's 1.7e-3).  T's inverse is f32 throughout, the running sum of g 64 bits,
+// since differences of a long sum are what the decays are made of.  The gated norm reads o in f32 from the workspace: rounded to the rows'
+// type before, fp16 rows had no o above 65504 and no bits in a small one, and the result of bf16 rows was half a step further off.
 #include "gdn.h"
 
 #include <algorithm>
@@ -20,6 +21,8 @@ namespace tsv {
 
 constexpr int BLK = 64, MS = 68;  // rows of a block; row stride (floats) of the 64 x 64 matrices in LDS
 constexpr int TFRAGS = 6;         // 16 x 32 fragments of a 64 x 64 lower triangle: row tile w has w / 2 + 1
+constexpr int TTILES = 10;        // 16 x 16 tiles of it: row tile w has w + 1
+constexpr int TP_UNITS = (TTILES + 2 * TFRAGS) * 64;  // 16-byte units of T in f32 tiles and P in fragments of two terms, of a (block, value head)
 
 struct PrefillArgs {
     const uint16_t *q, *k, *v;
@@ -45,6 +48,7 @@ template <int DK, int TR>
 constexpr int KFRAGS = 4 * (DK / 32) * TR;
 
 __device__ __host__ constexpr int tfrag(int w, int ks) { return w < 2 ? w : 2 * w - 2 + ks; }
+__device__ __host__ constexpr int ttile(int w, int j) { return w * (w + 1) / 2 + j; }
 
 // eight row values as one bf16 operand, or (fp16) two that sum to them exactly
 template <bool F16>
@@ -64,12 +68,15 @@ __device__ __forceinline__ void row_terms(const uint4& u, bf16x8* t) {
     }
 }
 
-// c += a b over terms: (1, 1), (1, 2) and (2, 1) whole, (2, 2) without lo * lo
+// c += a b over terms, without those products of two terms that are 2^-9 and less of the operands' own last terms
 template <int TA, int TB>
 __device__ __forceinline__ gf4 mfma_terms(const bf16x8* a, const bf16x8* b, gf4 c) {
-    c = mfma_bf16(a[0], b[0], c);
-    if constexpr (TB == 2) c = mfma_bf16(a[0], b[1], c);
-    if constexpr (TA == 2) c = mfma_bf16(a[1], b[0], c);
+    constexpr int MOST = TA > TB ? TA : TB;
+#pragma unroll
+    for (int i = 0; i < TA; i++)
+#pragma unroll
+        for (int j = 0; j < TB; j++)
+            if (i + j < MOST) c = mfma_bf16(a[i], b[j], c);
     return c;
 }
 
@@ -281,24 +288,27 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
             }
         }
         __syncthreads();
-        uint4* to = p.tp + ((int64_t)blk * sh.hv + h) * (TFRAGS * 4 * 64);
+        uint4* to = p.tp + ((int64_t)blk * sh.hv + h) * TP_UNITS;
+        const int row = 16 * w + l16;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (j > w) continue;
+            const int j0 = 16 * j + 4 * gq;
+            float4 x = *(const float4*)(T + row * MS + j0);  // (above the diagonal nothing has been written)
+            const float4 be = *(const float4*)(gt.beta + j0);
+            x.x = j0 <= row ? x.x * be.x : 0.0f;
+            x.y = j0 + 1 <= row ? x.y * be.y : 0.0f;
+            x.z = j0 + 2 <= row ? x.z * be.z : 0.0f;
+            x.w = j0 + 3 <= row ? x.w * be.w : 0.0f;
+            to[ttile(w, j) * 64 + lane] = __builtin_bit_cast(uint4, x);
+        }
 #pragma unroll
         for (int ks = 0; ks < 2; ks++) {
             if (ks > w / 2) continue;
-            const int f = tfrag(w, ks), j0 = 32 * ks + 8 * gq, row = 16 * w + l16;
-            uint4 th, tl;
-            float x[8];
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = j0 + e <= row ? T[row * MS + j0 + e] * gt.beta[j0 + e] : 0.0f;  // above the diagonal nothing has been written
-            split2(x[0], x[1], th.x, tl.x);
-            split2(x[2], x[3], th.y, tl.y);
-            split2(x[4], x[5], th.z, tl.z);
-            split2(x[6], x[7], th.w, tl.w);
-            to[(2 * f) * 64 + lane] = th;
-            to[(2 * f + 1) * 64 + lane] = tl;
+            const int f = tfrag(w, ks), j0 = 32 * ks + 8 * gq;
             const bool zero = 32 * ks + 8 * gq >= 16 * (w + 1);  // (columns of row tiles behind this one)
 #pragma unroll
-            for (int e = 0; e < 2; e++) to[(2 * TFRAGS + 2 * f + e) * 64 + lane] = zero ? make_uint4(0, 0, 0, 0) : *(const uint4*)(P + e * BLK * BLK + p_at(row, j0));
+            for (int e = 0; e < 2; e++) to[(TTILES + 2 * f + e) * 64 + lane] = zero ? make_uint4(0, 0, 0, 0) : *(const uint4*)(P + e * BLK * BLK + p_at(row, j0));
         }
         __syncthreads();
     }
@@ -306,8 +316,8 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
 
 // ---- the walk through a sequence's blocks --------------------------------------------------------------------------------------------
 // One workgroup of eight waves per (sequence, value head, 16 NT value channels).  Waves 0 to 3 take the state from block to block:
-// wave w owns rows 16 w .. of the block and k_dim / 4 rows of the state, which stay in its accumulators; the state, v - e^G kS and u
-// pass between them through LDS as bf16 terms in operand order, three barriers a block.  Waves 4 to 7, one beside each of them on a
+// wave w owns rows 16 w .. of the block and k_dim / 4 rows of the state, which stay in its accumulators; the state and u pass between
+// them through LDS as bf16 terms in operand order, v - e^G kS as the f32 instruction takes it, three barriers a block.  Waves 4 to 7, one beside each of them on a
 // SIMD, make the output rows from the same LDS (q S behind the first barrier, P u behind the third) and hand the others v, transposed,
 // and the decays through LDS: a load or store of any width holds the CU's address unit for 16 cycles, which bounds a block (12 and 9 of
 // them a wave here), so two-byte ones are taken together.  Everything a block reads is asked for one block ahead, into the registers
@@ -331,31 +341,31 @@ constexpr int walk_threads = NT == 1 && DK < 256 ? 576 : 512;
 template <int DK, bool F16, int NT>
 struct Walk {
     static constexpr int TR = F16 ? 2 : 1, KS = DK / 32, SD = DK / 64;
-    // LDS, all in operand order [k step][nt][term][lane]
-    static constexpr int S_AT = 0, R_AT = KS * NT * 2 * 64, U_AT = R_AT + 2 * NT * 2 * 64, D_AT = U_AT + 2 * NT * 2 * 64;
+    // LDS, in operand order [k step][nt][term][lane], but for the difference v - e^G kS, in f32 [row tile][nt][lane]
+    static constexpr int S_AT = 0, R_AT = KS * NT * 3 * 64, U_AT = R_AT + 4 * NT * 64, D_AT = U_AT + 2 * NT * 2 * 64;
     // v as [column][VS], the decays e^G and e^{G_end - G}, and the output rows on their way out, a region per wave (f32 rows of OS values)
-    static constexpr int V_AT = D_AT + 2 * NT * 2 * 64, VS = 72, G_AT = V_AT + 16 * NT * VS / 8, O_AT = G_AT + 32, OS = 16 * NT + 4, LDS = O_AT + 64 * OS / 4;
+    static constexpr int V_AT = D_AT + 2 * NT * 3 * 64, VS = 72, G_AT = V_AT + 16 * NT * VS / 8, O_AT = G_AT + 32, OS = 16 * NT + 4, LDS = O_AT + 64 * OS / 4;
     uint4* lds;
     int lane, w, l16, gq;
 
-    // four consecutive contraction indices of one column, as one or two terms, where the B operand's lane finds its eight
+    // four consecutive contraction indices of one column, as two or three terms, where the B operand's lane finds its eight
     template <int TERMS>
     __device__ __forceinline__ void put(int to, int step, int t, int group, gf4 x) const {
         uint2* f = (uint2*)(lds + to + (step * NT + t) * TERMS * 64) + (group * 16 + l16) * 2 + (gq & 1);
-        if (TERMS == 2) {
-            uint2 hi, lo;
-            split2(x[0], x[1], hi.x, lo.x);
-            split2(x[2], x[3], hi.y, lo.y);
-            f[0] = hi;
-            f[128] = lo;
-        } else {
-            f[0] = make_uint2(row_pair<false>(x[0], x[1]), row_pair<false>(x[2], x[3]));
+#pragma unroll
+        for (int e = 0; e < TERMS; e++) {
+            const uint2 two = make_uint2(row_pair<false>(x[0], x[1]), row_pair<false>(x[2], x[3]));
+            f[128 * e] = two;
+            x -= gf4{__uint_as_float(two.x << 16), __uint_as_float(two.x & 0xFFFF0000u), __uint_as_float(two.y << 16), __uint_as_float(two.y & 0xFFFF0000u)};
         }
     }
-    template <int TERMS>
+    // the same in f32, a tile of a product as it comes: one that the f32 instruction's contraction takes in rows 4 gq + r
+    __device__ __forceinline__ void put_f32(int to, int t, gf4 x) const { lds[to + (w * NT + t) * 64 + lane] = __builtin_bit_cast(uint4, x); }
+    // the first READ of an operand's terms
+    template <int TERMS, int READ = TERMS>
     __device__ __forceinline__ void get(int from, int step, int t, bf16x8* x) const {
 #pragma unroll
-        for (int e = 0; e < TERMS; e++) x[e] = __builtin_bit_cast(bf16x8, lds[from + ((step * NT + t) * TERMS + e) * 64 + lane]);
+        for (int e = 0; e < READ; e++) x[e] = __builtin_bit_cast(bf16x8, lds[from + ((step * NT + t) * TERMS + e) * 64 + lane]);
     }
 };
 
@@ -386,9 +396,9 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
     const float* ends = p.ends + ((int64_t)p.seg_of[s] * sh.hv + h) * (sh.dv + DK) * DK;  // of the sequence's first segment
     const int64_t ends_step = (int64_t)sh.hv * (sh.dv + DK) * DK;
     // uniform addresses of the block asked for, and what a lane adds to them (in bytes)
-    const char* tpp = (const char*)(p.tp + (b0 * sh.hv + h) * (TFRAGS * 4 * 64));
+    const char* tpp = (const char*)(p.tp + (b0 * sh.hv + h) * TP_UNITS);
     const char* gp = (const char*)(p.gates + (b0 * sh.hv + h) * 128);
-    const int64_t tp_step = (int64_t)sh.hv * (TFRAGS * 4 * 1024), g_step = (int64_t)sh.hv * 512;
+    const int64_t tp_step = (int64_t)sh.hv * (TP_UNITS * 16), g_step = (int64_t)sh.hv * 512;
     const uint32_t lane16 = lane * 16;
     // (waves of rows 0 and 16 have one fragment of T and P where the others have two: they ask for theirs twice and clear the copy, so
     // that every wave has the same loads under way and a wait is for the ones it needs)
@@ -398,8 +408,33 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         if (ks == 0) return __builtin_bit_cast(bf16x8, f);
         return __builtin_bit_cast(bf16x8, make_uint4(f.x & second, f.y & second, f.z & second, f.w & second));
     };
+    // u = T (v - e^G kS) of row tile i, columns of tile t, on the f32 instruction, and what is read of it
+    auto ask_t = [&](uint4* tr, int i) {  // (as many for every wave: row tile i has i + 1 tiles)
+#pragma unroll
+        for (int j = 0; j < 4; j++) tr[j] = *(const uint4*)(tpp + ttile(i, min(j, i)) * 1024 + lane16);
+    };
+    auto solve = [&](const uint4* tr, int i, int t) {
+        gf4 d[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) d[j] = __builtin_bit_cast(gf4, lds[W::R_AT + (j * NT + t) * 64 + lane]);
+        const gf4 ed = *(const gf4*)((const float*)(lds + W::G_AT) + 64 + 16 * i + 4 * gq);
+        GDN_FENCE;
+        gf4 u = {0, 0, 0, 0}, u2 = u;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            if (j > i) break;
+            const gf4 a = __builtin_bit_cast(gf4, tr[j]);
+            u = mfma_f32(a[0], d[j][0], u);
+            u2 = mfma_f32(a[1], d[j][1], u2);
+            u = mfma_f32(a[2], d[j][2], u);
+            u2 = mfma_f32(a[3], d[j][3], u2);
+        }
+        u += u2;
+        x.template put<3>(W::D_AT, i >> 1, t, 2 * (i & 1) + (gq >> 1), ed * u);
+        if constexpr (!ENDS) x.template put<2>(W::U_AT, i >> 1, t, 2 * (i & 1) + (gq >> 1), u);
+    };
     if (walk_threads<DK, NT> > 512 && w8 == 8) {  // ---- the wave that brings what is four blocks ahead into the XCD's L2, this workgroup's share of it
-        constexpr int AHEAD = 4, LINES = 3 * KFRAGS<DK, TR> * 8 + TFRAGS * 4 * 8, SHARE = 3;
+        constexpr int AHEAD = 4, LINES = 3 * KFRAGS<DK, TR> * 8 + TP_UNITS / 8, SHARE = 3;
         const char* kreg = (const char*)(p.kt + (b0 * sh.hk + hk) * (3 * KFRAGS<DK, TR> * 64));
         const int64_t k_step = (int64_t)sh.hk * (3 * KFRAGS<DK, TR> * 1024);
         const char* vreg = (const char*)(p.v + (int64_t)first * p.v_stride + h * sh.dv + (unit ? 0 : tile * 16 * NT));
@@ -429,7 +464,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
     if (w8 >= 4) {  // ---- the output's waves
         const char* qp = (const char*)(p.kt + ((b0 * sh.hk + hk) * 3 + 1) * (KFRAGS<DK, TR> * 64) + w * KS * TR * 64);
         const int64_t q_step = (int64_t)sh.hk * (3 * KFRAGS<DK, TR> * 1024);
-        uint4 qr[KS][TR], pr[2][2];
+        uint4 qr[KS][TR], pr[2][2], tr[4];  // (tr: of the row tile that this SIMD's other wave has least of)
         auto ask_q = [&]() {
 #pragma unroll
             for (int t = 0; t < KS; t++)
@@ -439,8 +474,8 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         auto ask_p = [&]() {
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-                pr[0][e] = *(const uint4*)(tpp + (2 * TFRAGS + 2 * f0 + e) * 1024 + lane16);
-                pr[1][e] = *(const uint4*)(tpp + (2 * TFRAGS + 2 * f1 + e) * 1024 + lane16);
+                pr[0][e] = *(const uint4*)(tpp + (TTILES + 2 * f0 + e) * 1024 + lane16);
+                pr[1][e] = *(const uint4*)(tpp + (TTILES + 2 * f1 + e) * 1024 + lane16);
             }
         };
         // a lane's piece of the rows: a quarter of row lane / 4 of the wave's sixteen
@@ -479,6 +514,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
                 ask_q();
                 ask_p();
             }
+            if constexpr (NT == 2) ask_t(tr, 3 - w);
             put_v();
             ask_v(1);
             GDN_ARRIVED;
@@ -490,6 +526,11 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
             __syncthreads();
             if constexpr (ENDS) {  // no rows go out: v and the decays alone
                 __syncthreads();
+                if constexpr (NT == 2) {
+                    solve(tr, 3 - w, 1);
+                    GDN_FENCE;
+                    ask_t(tr, 3 - w);
+                }
                 __syncthreads();
                 GDN_FENCE;
                 put_v();
@@ -501,7 +542,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
 #pragma unroll
             for (int i = 0; i < KS; i++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) x.template get<2>(W::S_AT, i, t, st[i][t]);
+                for (int t = 0; t < NT; t++) x.template get<3, 2>(W::S_AT, i, t, st[i][t]);
             const gf4 eg = *(const gf4*)((const float*)(lds + W::G_AT) + 16 * w + 4 * gq);
             GDN_FENCE;
             gf4 o[NT], o2[NT];
@@ -524,6 +565,11 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
             GDN_FENCE;
             __syncthreads();
             ask_q();
+            if constexpr (NT == 2) {
+                solve(tr, 3 - w, 1);
+                GDN_FENCE;
+                ask_t(tr, 3 - w);
+            }
             __syncthreads();
             bf16x8 u[2][NT][2];
 #pragma unroll
@@ -595,7 +641,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
     const char* kp = (const char*)(p.kt + (b0 * sh.hk + hk) * (3 * KFRAGS<DK, TR> * 64) + w * KS * TR * 64);
     const char* ktp = (const char*)(p.kt + ((b0 * sh.hk + hk) * 3 + 2) * (KFRAGS<DK, TR> * 64) + SD * w * 2 * TR * 64);
     const int64_t k_step = (int64_t)sh.hk * (3 * KFRAGS<DK, TR> * 1024);
-    uint4 kr[KS][TR], ktr[SD][2][TR], tr[2][2];
+    uint4 kr[KS][TR], ktr[SD][2][TR], tr[4];
     const uint16_t* vt = (const uint16_t*)(lds + W::V_AT) + l16 * W::VS + 16 * w + 4 * gq;
     const float* gates = (const float*)(lds + W::G_AT);
     auto ask_k = [&]() {
@@ -603,13 +649,6 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         for (int t = 0; t < KS; t++)
 #pragma unroll
             for (int e = 0; e < TR; e++) kr[t][e] = *(const uint4*)(kp + (t * TR + e) * 1024 + lane16);
-    };
-    auto ask_t = [&]() {
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            tr[0][e] = *(const uint4*)(tpp + (2 * f0 + e) * 1024 + lane16);
-            tr[1][e] = *(const uint4*)(tpp + (2 * f1 + e) * 1024 + lane16);
-        }
     };
     auto ask_kt = [&]() {
 #pragma unroll
@@ -623,7 +662,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
 #pragma unroll
         for (int d = 0; d < SD; d++)
 #pragma unroll
-            for (int t = 0; t < NT; t++) x.template put<2>(W::S_AT, (SD * w + d) >> 1, t, 2 * ((SD * w + d) & 1) + (gq >> 1), S[d][t]);
+            for (int t = 0; t < NT; t++) x.template put<3>(W::S_AT, (SD * w + d) >> 1, t, 2 * ((SD * w + d) & 1) + (gq >> 1), S[d][t]);
     };
     if constexpr (!ENDS)
         for (int q = 0; q < seg; q++) {  // the segments before this one: S <- M S + c
@@ -642,17 +681,17 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
                 for (int t = 0; t < NT; t++) S[d][t] = *(const gf4*)(c + (int64_t)(tile * 16 * NT + 16 * t + l16) * DK + 16 * (SD * w + d) + 4 * gq);
 #pragma unroll
                 for (int i = 0; i < KS; i++) {
-                    uint4 hi, lo;
-                    split2(m[i][0].x, m[i][0].y, hi.x, lo.x);
-                    split2(m[i][0].z, m[i][0].w, hi.y, lo.y);
-                    split2(m[i][1].x, m[i][1].y, hi.z, lo.z);
-                    split2(m[i][1].z, m[i][1].w, hi.w, lo.w);
-                    const bf16x8 a[2] = {__builtin_bit_cast(bf16x8, hi), __builtin_bit_cast(bf16x8, lo)};
+                    uint4 m3[3];
+                    split3(m[i][0].x, m[i][0].y, m3[0].x, m3[1].x, m3[2].x);
+                    split3(m[i][0].z, m[i][0].w, m3[0].y, m3[1].y, m3[2].y);
+                    split3(m[i][1].x, m[i][1].y, m3[0].z, m3[1].z, m3[2].z);
+                    split3(m[i][1].z, m[i][1].w, m3[0].w, m3[1].w, m3[2].w);
+                    const bf16x8 a[3] = {__builtin_bit_cast(bf16x8, m3[0]), __builtin_bit_cast(bf16x8, m3[1]), __builtin_bit_cast(bf16x8, m3[2])};
 #pragma unroll
                     for (int t = 0; t < NT; t++) {
-                        bf16x8 st[2];
-                        x.template get<2>(W::S_AT, i, t, st);
-                        S[d][t] = mfma_terms<2, 2>(a, st, S[d][t]);
+                        bf16x8 st[3];
+                        x.template get<3>(W::S_AT, i, t, st);
+                        S[d][t] = mfma_terms<3, 3>(a, st, S[d][t]);
                     }
                 }
             }
@@ -660,7 +699,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         }
     if (blocks > 0) {
         ask_k();
-        ask_t();
+        ask_t(tr, w);
         ask_kt();
         put_state();
         GDN_ARRIVED;
@@ -672,29 +711,37 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         tpp += more ? tp_step : 0;
         __syncthreads();
         {
-            bf16x8 st[KS][NT][2];
-#pragma unroll
-            for (int i = 0; i < KS; i++)
-#pragma unroll
-                for (int t = 0; t < NT; t++) x.template get<2>(W::S_AT, i, t, st[i][t]);
             uint2 v4[NT];
 #pragma unroll
             for (int t = 0; t < NT; t++) v4[t] = *(const uint2*)(vt + 16 * t * W::VS);
             const gf4 eg = *(const gf4*)(gates + 16 * w + 4 * gq);
-            GDN_FENCE;
             gf4 c[NT], c2[NT];
 #pragma unroll
             for (int t = 0; t < NT; t++) c[t] = c2[t] = gf4{0, 0, 0, 0};
+            constexpr int PART = KS > 4 ? KS / 2 : KS;  // (k_dim 256 has no registers for all of the state's terms at once)
 #pragma unroll
-            for (int i = 0; i < KS; i++) {
-                bf16x8 a[TR];
+            for (int i0 = 0; i0 < KS; i0 += PART) {
+                bf16x8 st[PART][NT][3];
 #pragma unroll
-                for (int e = 0; e < TR; e++) a[e] = __builtin_bit_cast(bf16x8, kr[i][e]);
+                for (int i = 0; i < PART; i++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    c[t] = mfma_bf16(a[0], st[i][t][0], c[t]);
-                    c2[t] = mfma_bf16(a[0], st[i][t][1], c2[t]);
-                    if constexpr (TR == 2) c2[t] = mfma_bf16(a[1], st[i][t][0], c2[t]);
+                    for (int t = 0; t < NT; t++) x.template get<3>(W::S_AT, i0 + i, t, st[i][t]);
+                GDN_FENCE;
+#pragma unroll
+                for (int i = 0; i < PART; i++) {
+                    bf16x8 a[TR];
+#pragma unroll
+                    for (int e = 0; e < TR; e++) a[e] = __builtin_bit_cast(bf16x8, kr[i0 + i][e]);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) {
+                        c[t] = mfma_bf16(a[0], st[i][t][0], c[t]);
+                        c2[t] = mfma_bf16(a[0], st[i][t][1], c2[t]);
+                        c2[t] = mfma_bf16(a[0], st[i][t][2], c2[t]);
+                        if constexpr (TR == 2) {
+                            c2[t] = mfma_bf16(a[1], st[i][t][0], c2[t]);
+                            c2[t] = mfma_bf16(a[1], st[i][t][1], c2[t]);
+                        }
+                    }
                 }
             }
 #pragma unroll
@@ -702,40 +749,16 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
                 gf4 d;
 #pragma unroll
                 for (int r = 0; r < 4; r++) d[r] = fmaf(-eg[r], c[t][r] + c2[t][r], row_f32<F16>((uint16_t)((r & 2 ? v4[t].y : v4[t].x) >> (16 * (r & 1)))));
-                x.template put<2>(W::R_AT, w >> 1, t, 2 * (w & 1) + (gq >> 1), d);
+                x.put_f32(W::R_AT, t, d);
             }
         }
         __syncthreads();
         {
-            bf16x8 d[2][NT][2];
-#pragma unroll
-            for (int ks = 0; ks < 2; ks++)
-#pragma unroll
-                for (int t = 0; t < NT; t++) x.template get<2>(W::R_AT, ks, t, d[ks][t]);
-            GDN_FENCE;
-            const gf4 ed = *(const gf4*)(gates + 64 + 16 * w + 4 * gq);
             const float e_end = gates[63];
             ask_k();
             GDN_FENCE;
-            gf4 u[NT], u2[NT];
-#pragma unroll
-            for (int t = 0; t < NT; t++) u[t] = u2[t] = gf4{0, 0, 0, 0};
-#pragma unroll
-            for (int ks = 0; ks < 2; ks++) {
-                const bf16x8 a0 = fragment(tr[ks][0], ks), a1 = fragment(tr[ks][1], ks);
-#pragma unroll
-                for (int t = 0; t < NT; t++) {
-                    u[t] = mfma_bf16(a0, d[ks][t][0], u[t]);
-                    u2[t] = mfma_bf16(a0, d[ks][t][1], u2[t]);
-                    u2[t] = mfma_bf16(a1, d[ks][t][0], u2[t]);
-                }
-            }
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-                u[t] += u2[t];
-                x.template put<2>(W::D_AT, w >> 1, t, 2 * (w & 1) + (gq >> 1), ed * u[t]);
-                if constexpr (!ENDS) x.template put<2>(W::U_AT, w >> 1, t, 2 * (w & 1) + (gq >> 1), u[t]);
-            }
+            // (two column tiles: the second's is the other wave's of a SIMD, row tiles the other way round, so that every SIMD has as many products)
+            solve(tr, w, 0);
 #pragma unroll
             for (int i = 0; i < SD; i++)
 #pragma unroll
@@ -743,13 +766,13 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         }
         __syncthreads();
         {
-            bf16x8 d[2][NT][2];
+            bf16x8 d[2][NT][3];
 #pragma unroll
             for (int ks = 0; ks < 2; ks++)
 #pragma unroll
-                for (int t = 0; t < NT; t++) x.template get<2>(W::D_AT, ks, t, d[ks][t]);
+                for (int t = 0; t < NT; t++) x.template get<3>(W::D_AT, ks, t, d[ks][t]);
             GDN_FENCE;
-            ask_t();
+            ask_t(tr, w);
             GDN_FENCE;
 #pragma unroll
             for (int ks = 0; ks < 2; ks++)
@@ -759,7 +782,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
 #pragma unroll
                     for (int e = 0; e < TR; e++) a[e] = __builtin_bit_cast(bf16x8, ktr[i][ks][e]);
 #pragma unroll
-                    for (int t = 0; t < NT; t++) S[i][t] = mfma_terms<TR, 2>(a, d[ks][t], S[i][t]);
+                    for (int t = 0; t < NT; t++) S[i][t] = mfma_terms<TR, 3>(a, d[ks][t], S[i][t]);
                 }
         }
         ask_kt();
@@ -846,7 +869,7 @@ Sizes workspace_of(const GdnShape& sh, const GdnBatch& bt, int dk, bool f16) {
         z.segments += std::max<int64_t>(1, (blocks_of(bt, s) + z.seg_blocks - 1) / z.seg_blocks);
     }
     z.kt = z.blocks * sh.hk * (3 * (dk / 8) * tr * 1024);
-    z.tp = z.blocks * sh.hv * (TFRAGS * 4 * 1024);
+    z.tp = z.blocks * sh.hv * (TP_UNITS * 16);
     z.gates = z.blocks * sh.hv * 512;
     z.ends = z.seg_blocks == INT32_MAX ? 0 : z.segments * sh.hv * (sh.dv + dk) * dk * 4;
     z.starts = z.seg_blocks == INT32_MAX ? 0 : (int64_t)bt.n_seq * sh.hv * sh.dv * dk * 4;
