@@ -7,8 +7,8 @@
 // sequence with 16 NT columns of one head's state in registers, k_gdn_norm is the gated norm of the result.
 //
 // Precision: the state is f32 and never rounded.  In what makes it, k S and k^T u, it and u are three bf16 terms each (2^-27, split3), k the
-// rows' own bits (fp16 rows: two terms, exact); T (v - e^G kS) is made by the f32 instruction from f32 operands.  The state is then as far
-// off as one of plain 32-bit sums, 2e-7 to 1e-6 of its norm after thousands of rows (two terms throughout: 5e-6; one would leave 2e-3).
+// rows' own bits (fp16 rows: two terms, exact); k k^T is made of the rows' bits as they are, T (v - e^G kS) by the f32 instruction from f32
+// operands.  The state is then as far off as one of plain 32-bit sums, 1.2e-7 to 1.5e-7 of its norm (two terms throughout: 5e-6).
 // What only goes to the output, q S and P u, has two terms by two (2^-18, split2), so that the rows' own rounding is what a result is off by
 // (P u one term by one left bf16 rows 2.6e-3 off for their rounding's 1.7e-3).  T's inverse is f32 throughout, the running sum of g 64 bits,
 // since differences of a long sum are what the decays are made of.  The gated norm reads o in f32 from the workspace: rounded to the rows'
@@ -80,6 +80,14 @@ __device__ __forceinline__ gf4 mfma_terms(const bf16x8* a, const bf16x8* b, gf4 
     return c;
 }
 
+// the product of the rows' own bits
+template <bool F16>
+__device__ __forceinline__ gf4 mfma_rows(const uint4& a, const uint4& b, gf4 c) {
+    typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+    if constexpr (F16) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else return mfma_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
+}
+
 __device__ __forceinline__ int sequence_of(const int32_t* starts, int n, int at) {
     int lo = 0, hi = n;
     while (hi - lo > 1) {
@@ -100,9 +108,9 @@ __device__ __forceinline__ int sequence_of(const int32_t* starts, int n, int at)
 // Where P's value (i, j) lies in LDS: rows of 64 values, whose eight 16-byte units take turns from row to row (a column of them, as the
 // fragments are read, would else lie in two banks)
 __device__ __forceinline__ int p_at(int i, int j) { return i * BLK + (((j >> 3) ^ (i & 7)) << 3) + (j & 7); }
-// 16-byte units of LDS that hold k's operands, then P
-template <int DK, int TR>
-constexpr int blocks_operands = KFRAGS<DK, TR> * 64 > 2 * BLK * BLK / 8 ? KFRAGS<DK, TR> * 64 : 2 * BLK * BLK / 8;
+// 16-byte units of LDS that hold k's rows, then P
+template <int DK>
+constexpr int blocks_operands = DK > 2 * BLK ? BLK * DK / 8 : 2 * BLK * BLK / 8;
 
 // What a head's decays are in a block.  e^{G_i - G_j} of rows in different row tiles is made of three factors of at most 1: from j to its
 // tile's end, the tiles between, and from the start of i's tile to i; inside a tile it is one exponential of a 64-bit difference.
@@ -117,9 +125,9 @@ template <int DK, bool F16>
 __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt, PrefillArgs p) {
     constexpr int TR = F16 ? 2 : 1, KS = DK / 32;
     extern __shared__ uint4 lds[];
-    uint4* kf = lds;                                   // [row tile][k step][term][lane]
+    uint4* kf = lds;                                   // [row tile][k step][lane], as the rows have them
     uint16_t* P = (uint16_t*)lds;                      // [term][64][64], where the operands were
-    float* A = (float*)(lds + blocks_operands<DK, TR>);  // [64][MS]
+    float* A = (float*)(lds + blocks_operands<DK>);  // [64][MS]
     float* T = A + BLK * MS;
     BlockGates* gates = (BlockGates*)(T + BLK * MS);   // of GATE_HEADS heads
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, gq = lane >> 4;
@@ -136,53 +144,56 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
         next_b = p.beta[at];
     };
     ask_gates(h0 + w);
-    bf16x8 kr[KS][TR], qr[KS][TR];
+    uint4 kr[KS], qr[KS];
     uint4* rows_out = p.kt + ((int64_t)blk * sh.hk + hk) * (3 * KFRAGS<DK, TR> * 64);
 #pragma unroll
     for (int t = 0; t < KS; t++) {
-        uint4 a = make_uint4(0, 0, 0, 0), b = a;
+        kr[t] = qr[t] = make_uint4(0, 0, 0, 0);
         if (mine < n) {
-            a = *(const uint4*)(p.k + (row0 + mine) * p.k_stride + hk * DK + 32 * t + 8 * gq);
-            b = *(const uint4*)(p.q + (row0 + mine) * p.q_stride + hk * DK + 32 * t + 8 * gq);
+            kr[t] = *(const uint4*)(p.k + (row0 + mine) * p.k_stride + hk * DK + 32 * t + 8 * gq);
+            qr[t] = *(const uint4*)(p.q + (row0 + mine) * p.q_stride + hk * DK + 32 * t + 8 * gq);
         }
-        row_terms<F16>(a, kr[t]);
-        row_terms<F16>(b, qr[t]);
+        kf[(w * KS + t) * 64 + lane] = kr[t];
+        if (!writes) continue;
+        bf16x8 k[TR], q[TR];
+        row_terms<F16>(kr[t], k);
+        row_terms<F16>(qr[t], q);
 #pragma unroll
         for (int e = 0; e < TR; e++) {
             const int f = (w * KS + t) * TR + e;
-            kf[f * 64 + lane] = __builtin_bit_cast(uint4, kr[t][e]);
-            if (writes) rows_out[f * 64 + lane] = __builtin_bit_cast(uint4, kr[t][e]);
-            if (writes) rows_out[(KFRAGS<DK, TR> + f) * 64 + lane] = __builtin_bit_cast(uint4, qr[t][e]);
+            rows_out[f * 64 + lane] = __builtin_bit_cast(uint4, k[e]);
+            rows_out[(KFRAGS<DK, TR> + f) * 64 + lane] = __builtin_bit_cast(uint4, q[e]);
         }
     }
     __syncthreads();
-    gf4 kk[4], qk[4];
+    gf4 kk[4], qk[4];  // of the rows' own bits: exact products
 #pragma unroll
     for (int c = 0; c < 4; c++) {
         kk[c] = qk[c] = gf4{0, 0, 0, 0};
         if (c > w) continue;
 #pragma unroll
         for (int t = 0; t < KS; t++) {
-            bf16x8 b[TR];
-#pragma unroll
-            for (int e = 0; e < TR; e++) b[e] = __builtin_bit_cast(bf16x8, kf[((c * KS + t) * TR + e) * 64 + lane]);
-            kk[c] = mfma_terms<TR, TR>(kr[t], b, kk[c]);
-            qk[c] = mfma_terms<TR, TR>(qr[t], b, qk[c]);
+            const uint4 b = kf[(c * KS + t) * 64 + lane];
+            kk[c] = mfma_rows<F16>(kr[t], b, kk[c]);
+            qk[c] = mfma_rows<F16>(qr[t], b, qk[c]);
         }
     }
     // k transposed, as the operand of the state's update: rows k_dim, eight block rows a lane
     if (writes) {
         const uint16_t* kh = (const uint16_t*)kf;
         uint4* to = rows_out + 2 * KFRAGS<DK, TR> * 64;
-        for (int f = w; f < DK / 16 * 2 * TR; f += 4) {
-            const int e = f % TR, ks = f / TR % 2, d = 16 * (f / TR / 2) + l16;
+        for (int f = w; f < DK / 16 * 2; f += 4) {
+            const int ks = f % 2, d = 16 * (f / 2) + l16;
             uint16_t x[8];
 #pragma unroll
             for (int i = 0; i < 8; i++) {
                 const int row = 32 * ks + 8 * gq + i;
-                x[i] = kh[((((row >> 4) * KS + (d >> 5)) * TR + e) * 64 + ((d & 31) >> 3) * 16 + (row & 15)) * 8 + (d & 7)];
+                x[i] = kh[(((row >> 4) * KS + (d >> 5)) * 64 + ((d & 31) >> 3) * 16 + (row & 15)) * 8 + (d & 7)];
             }
-            to[f * 64 + lane] = make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16);
+            bf16x8 k[TR];
+            row_terms<F16>(make_uint4(x[0] | (uint32_t)x[1] << 16, x[2] | (uint32_t)x[3] << 16, x[4] | (uint32_t)x[5] << 16, x[6] | (uint32_t)x[7] << 16), k);
+#pragma unroll
+            for (int e = 0; e < TR; e++) to[(f * TR + e) * 64 + lane] = __builtin_bit_cast(uint4, k[e]);
         }
     }
     for (int h = h0; h < h1; h++) {
@@ -880,8 +891,7 @@ Sizes workspace_of(const GdnShape& sh, const GdnBatch& bt, int dk, bool f16) {
 
 template <int DK, bool F16>
 int launch_blocks(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, PrefillArgs& p, int blocks) {
-    constexpr int TR = F16 ? 2 : 1;
-    const size_t lds = (size_t)blocks_operands<DK, TR> * 16 + 2 * BLK * MS * 4 + GATE_HEADS * sizeof(BlockGates);
+    const size_t lds = (size_t)blocks_operands<DK> * 16 + 2 * BLK * MS * 4 + GATE_HEADS * sizeof(BlockGates);
     static OncePerDevice once;
     const int rc = allow_lds((const void*)k_gdn_blocks<DK, F16>, lds, once);
     if (rc) return rc;
