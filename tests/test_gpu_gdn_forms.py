@@ -159,3 +159,16 @@ def test_a_norm_of_several_launches():
         want = ly.gate(o[None], z).reshape(-1)
         assert np.linalg.norm(from_bits(got, HF) - want) <= 4 * half_step(HF) * np.linalg.norm(want), row
     assert np.array_equal(dstate.get(), state)
+
+
+@pytest.mark.parametrize("lengths", [[1, 2100, 0], [0, 0, 2049, 64, 1, 65, 3]])
+def test_a_long_prompt_in_segments_beside_short_ones(lengths):
+    rng = np.random.default_rng(len(lengths))
+    ly = Layer(rng, 2, 8, 64, 128, 4, BF)
+    assert len(lengths) * ly.hv * ly.dv // 16 > 64 >= ly.hv * ly.dv // 16 and max(blocks_of(lengths)) >= 32
+    p = Prompt(rng, ly, lengths, [3 * (s % 2) for s in range(len(lengths))], gated=True)
+    ly.gpu.prefill(p.batch, p.io)
+    got, S = p.check()
+    p.io.state_out = p.io.state_in
+    ly.gpu.prefill(p.batch, p.io)
+    assert np.array_equal(p.out.get(), got) and np.array_equal(p.din.get(), S)

@@ -152,3 +152,31 @@ def test_offsets_are_whole_numbers_that_fit():
                 np.array([0, (1 << 64) - 1], np.uint64), [], 3):
         with pytest.raises(ValueError):
             layer.batch(bad, P)
+
+
+def _segments(layer, offsets):
+    """How many segments a batch is walked in, from what the workspace has beside its blocks' part: 0 where sequences are walked whole."""
+    L = ffi.lib()
+    size = lambda off: L.tsv_gdn_prefill_workspace(C.byref(layer), C.byref(_batch(offsets=off)))  # noqa: E731
+    blocks = sum(-(-(b - a) // 64) for a, b in zip(offsets, offsets[1:]))
+    more = size(offsets) - blocks * size((0, 64))
+    state = 4 * layer.n_v_heads * layer.v_dim * layer.k_dim
+    segment = 4 * layer.n_v_heads * (layer.v_dim + layer.k_dim) * layer.k_dim
+    n = len(offsets) - 1                          # a sequence's last segment leaves nothing for others
+    return (more - n * state) / segment + n if more else 0
+
+
+def test_segments_go_by_the_long_sequences():
+    few = _layer(n_k_heads=4, n_v_heads=8, k_dim=128, v_dim=128)
+    assert _segments(few, (0, 32768)) == 8
+    # short sequences beside the long one do not take it out of its segments
+    assert _segments(few, (0, 32768, 32769)) == 9 and _segments(few, (0, 0, 0, 32768, 32768)) == 11
+    assert _segments(few, (0, 130, 32768 + 130, 32768 + 200)) == 10
+    # as many long ones as fill the compute units do, and so do more heads
+    assert _segments(few, (0, 32768, 65536)) == 0 and _segments(few, (0, 32768, 32768 + 20000)) == 0
+    assert _segments(_layer(n_k_heads=4, n_v_heads=16, k_dim=128, v_dim=128), (0, 32768)) == 0
+    assert _segments(few, (0, 64 * 31)) == 0 and _segments(few, (0, 64 * 31 + 1)) > 0
+    # one narrow head: no more segments than putting them together is worth
+    narrow = _layer(n_k_heads=1, n_v_heads=1, k_dim=128, v_dim=16)
+    assert 32 <= _segments(narrow, (0, 1 << 18)) <= 64
+    assert _segments(narrow, (0, 4096)) <= 8

@@ -16,6 +16,7 @@
 #include "gdn.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace tsv {
 
@@ -34,7 +35,7 @@ struct PrefillArgs {
     int64_t out_stride;
     uint4 *kt, *tp;  // workspace: k, q and k transposed per (block, key head); T and P fragments per (block, value head)
     float* gates;    // ... and e^G, e^{G_end - G}
-    float* ends;     // ... and per (segment, value head) what a segment does to a state: [v_dim][k_dim] from nothing, then [k_dim][k_dim]
+    float* ends;     // ... and per (segment but a sequence's last, value head) what a segment does to a state: [v_dim][k_dim] from nothing, then [k_dim][k_dim]
     float* starts;   // ... and the states that sequences of several segments start from: state_out may be state_in
     float* o32;      // ... and the rows of o that the gated norm reads
     int32_t tiles;   // column tiles of a head in the walk
@@ -404,7 +405,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
     const int rows = last ? bt.off[s + 1] - first : p.seg_blocks * BLK, blocks = (rows + BLK - 1) / BLK;
     const int64_t b0 = p.block_of[s] + skip;
     const bool unit = ENDS && tile * 16 * NT >= sh.dv;  // columns of the unit matrix, not of the rows' v
-    const float* ends = p.ends + ((int64_t)p.seg_of[s] * sh.hv + h) * (sh.dv + DK) * DK;  // of the sequence's first segment
+    const float* ends = p.ends + ((int64_t)(p.seg_of[s] - s) * sh.hv + h) * (sh.dv + DK) * DK;  // of the sequence's first segment
     const int64_t ends_step = (int64_t)sh.hv * (sh.dv + DK) * DK;
     // uniform addresses of the block asked for, and what a lane adds to them (in bytes)
     const char* tpp = (const char*)(p.tp + (b0 * sh.hv + h) * TP_UNITS);
@@ -800,7 +801,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         put_state();
     }
     if constexpr (ENDS) {
-        float* to = p.ends + ((int64_t)seg_at * sh.hv + h) * (sh.dv + DK) * DK;
+        float* to = p.ends + ((int64_t)(seg_at - s) * sh.hv + h) * (sh.dv + DK) * DK;
 #pragma unroll
         for (int d = 0; d < SD; d++)
 #pragma unroll
@@ -853,14 +854,20 @@ int64_t blocks_of(const GdnBatch& bt, int s) { return (bt.off[s + 1] - bt.off[s]
 
 // How many blocks a segment has, INT32_MAX: whole sequences.  In segments a sequence's columns are walked twice and the k_dim columns of the
 // unit matrix once, so that it pays where at most a quarter of the compute units would have a workgroup: 32768 rows of 8 heads of 128
-// (64 column tiles) take 596 us whole, 338 in 4 segments (157 for M and c, 181), 290 in 8 (157 and 133), 331 in 16 (163 and 168).
-// Segments of fewer than 8 blocks gain nothing over what putting them together takes (2.5 us each).
+// (64 column tiles) take 817 us whole, 515 in 4 segments, 465 in 8 and 515 in 16.  Sequences count by their length beside the longest: short
+// ones are done early (one row beside those 32768: 457 us in 8 segments, 819 whole).  Segments of fewer than 8 blocks gain nothing over
+// what putting them together takes, and since each puts together all before it, which takes as long as a block or two, there are no more
+// than the square root of the blocks (262144 rows of one head of 16: 601 us in 64, 2274 in 512).
 int segment_blocks(const GdnShape& sh, const GdnBatch& bt) {
-    int64_t longest = 0;
-    for (int s = 0; s < bt.n_seq; s++) longest = std::max(longest, blocks_of(bt, s));
-    const int64_t tiles = (int64_t)bt.n_seq * sh.hv * (sh.dv / 16);
-    if (tiles > 64 || longest < 32) return INT32_MAX;
-    const int64_t segs = std::min<int64_t>(512 / tiles, longest / 8);
+    int64_t longest = 0, all = 0;
+    for (int s = 0; s < bt.n_seq; s++) {
+        longest = std::max(longest, blocks_of(bt, s));
+        all += blocks_of(bt, s);
+    }
+    if (longest < 32) return INT32_MAX;
+    const int64_t tiles = (2 * all + longest) / (2 * longest) * sh.hv * (sh.dv / 16);
+    if (tiles > 64) return INT32_MAX;
+    const int64_t segs = std::min({512 / tiles, longest / 8, (int64_t)sqrt((double)longest)});
     return (int)((longest + segs - 1) / segs);
 }
 
@@ -882,7 +889,7 @@ Sizes workspace_of(const GdnShape& sh, const GdnBatch& bt, int dk, bool f16) {
     z.kt = z.blocks * sh.hk * (3 * (dk / 8) * tr * 1024);
     z.tp = z.blocks * sh.hv * (TP_UNITS * 16);
     z.gates = z.blocks * sh.hv * 512;
-    z.ends = z.seg_blocks == INT32_MAX ? 0 : z.segments * sh.hv * (sh.dv + dk) * dk * 4;
+    z.ends = z.seg_blocks == INT32_MAX ? 0 : (z.segments - bt.n_seq) * sh.hv * (sh.dv + dk) * dk * 4;
     z.starts = z.seg_blocks == INT32_MAX ? 0 : (int64_t)bt.n_seq * sh.hv * sh.dv * dk * 4;
     z.o32 = sh.norm ? z.blocks * BLK * sh.hv * sh.dv * 4 : 0;  // (without norm weights a layer has no gated norm)
     z.total = z.kt + z.tp + z.gates + z.ends + z.starts + z.o32;
