@@ -465,7 +465,8 @@ int64_t tsv_vocab(const tsv_ctx* ctx);
  * States: f32, n_seq x n_v_heads x v_dim x k_dim (one run of k_dim per value channel), 16-byte aligned.  The convolution's
  * state is a ring of TSV_GDN_RING raw projection rows a sequence (n_seq x TSV_GDN_RING x channels, the rows' type): position p
  * lies in slot p % TSV_GDN_RING, so that nothing has to be erased when a pass is rejected.  A sequence whose base is 0 starts
- * from nothing, whatever its state and ring hold.
+ * from nothing, whatever its state and ring hold.  Calls write a state_out whole but of a ring_out the slots of their own rows only: one
+ * other than ring_in has to hold a copy of ring_in before the call, since later calls read rows behind those of this one too.
  *
  * Rows are bf16 or fp16.  Strides are elements from row to row, multiples of 8, at most 2^22; qkv, q, k, v, z, out and the rings are 16-byte
  * aligned.  Rows outside the batch's sequences are neither read nor written.  A row that holds no number spoils its own sequence: the
@@ -483,7 +484,7 @@ typedef struct {
     /* device, f32: channels x conv_width; n_v_heads; n_v_heads; v_dim (NULL where the call does not need it) */
     const float *conv, *a_log, *dt_bias, *norm;
 } tsv_gdn_layer;
-/* The rows of a call: sequence s owns rows [offsets[s], offsets[s + 1]); a sequence without rows keeps its state. */
+/* The rows of a call: sequence s owns rows [offsets[s], offsets[s + 1]); a sequence without rows keeps its state and ring. */
 typedef struct {
     int32_t n_seq;          /* 1..TSV_GDN_MAX_SEQ */
     const int32_t* offsets; /* HOST, n_seq + 1, from 0, not decreasing: the shape of the launches */
@@ -495,7 +496,7 @@ typedef struct {
 
 /* The convolution's part for prompts: out gets channels values a row (unit q, unit k, v) in the rows' type, g and beta (f32,
  * rows x n_v_heads) the decays and betas; the last conv_width - 1 rows of every sequence go to its ring.  Slots of ring_out that
- * no row goes to are left as they are (ring_out other than ring_in: a pass that can be made again from the same rings). */
+ * no row goes to are left as they are (a ring_out other than ring_in, a copy of it: a pass that can be made again from the same rings). */
 typedef struct {
     const void* qkv;
     int64_t qkv_stride;
@@ -558,7 +559,7 @@ int32_t tsv_gdn_step(void* stream, const tsv_gdn_layer* layer, const tsv_gdn_bat
  * that of the steps (its parent is not read), results the tsv_round_result of every sequence in DEVICE memory, as
  * tsv_accept_greedy_noalloc leaves it; record, states and rings are the first layer's, the strides lead from layer to layer
  * (record_stride in bytes, a multiple of 4; ring_stride and state_stride in elements, multiples of 8 and 4).  Slots of ring_out
- * that no kept row goes to are left as they are. */
+ * that no kept row goes to are left as they are: one other than ring_in has to be a copy of it. */
 typedef struct {
     int32_t n_layers;
     const tsv_round_result* results;

@@ -233,7 +233,8 @@ class GdnBatch(C.Structure):
 
 
 class GdnConv(C.Structure):
-    """tsv_gdn_conv_io: device addresses, strides in elements.  `ring` stands for ring_in and ring_out, a ring that is updated in place."""
+    """tsv_gdn_conv_io: device addresses, strides in elements.  `ring` stands for ring_in and ring_out, a ring that is updated in place; a
+    ring_out of its own has to hold a copy of ring_in, since a call writes the slots of its own rows only."""
     _fields_ = [("qkv", C.c_void_p), ("qkv_stride", C.c_int64), ("a", C.c_void_p), ("b", C.c_void_p), ("gate_stride", C.c_int64),
                 ("ring_in", C.c_void_p), ("ring_out", C.c_void_p), ("out", C.c_void_p), ("out_stride", C.c_int64), ("g", C.c_void_p),
                 ("beta", C.c_void_p)]
@@ -270,7 +271,7 @@ class GdnStep(C.Structure):
 
 
 class GdnCommit(C.Structure):
-    """tsv_gdn_commit_io"""
+    """tsv_gdn_commit_io.  A ring_out other than ring_in has to hold a copy of it, as with GdnConv."""
     _fields_ = [("n_layers", C.c_int32), ("results", C.c_void_p), ("record", C.c_void_p), ("record_stride", C.c_int64),
                 ("ring_in", C.c_void_p), ("ring_out", C.c_void_p), ("ring_stride", C.c_int64), ("state_in", C.c_void_p),
                 ("state_out", C.c_void_p), ("state_stride", C.c_int64)]
