@@ -172,3 +172,19 @@ def test_a_long_prompt_in_segments_beside_short_ones(lengths):
     p.io.state_out = p.io.state_in
     ly.gpu.prefill(p.batch, p.io)
     assert np.array_equal(p.out.get(), got) and np.array_equal(p.din.get(), S)
+
+
+@pytest.mark.parametrize("gated", [True, False])
+def test_blocks_brought_into_the_cache_ahead(gated):
+    """fp16 rows of k_dim 128 whose blocks' matrices are 128 MB and more: the walk has a ninth wave."""
+    rng = np.random.default_rng(16)
+    ly = Layer(rng, 32, 32, 128, 16, 4, HF)
+    lengths = [900, 1300, 1, 64, 0]
+    per_block = 32 * 3 * 128 // 8 * 2 * 1024 + 32 * 22 * 1024
+    assert sum(blocks_of(lengths)) * per_block >= 128 << 20
+    p = Prompt(rng, ly, lengths, [0, 3, 2, 0, 1], gated=gated)
+    ly.gpu.prefill(p.batch, p.io)
+    rows, S = p.check()
+    p.io.state_out = p.io.state_in
+    ly.gpu.prefill(p.batch, p.io)
+    assert np.array_equal(p.out.get(), rows) and np.array_equal(p.din.get(), S)

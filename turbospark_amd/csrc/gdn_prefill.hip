@@ -39,6 +39,7 @@ struct PrefillArgs {
     float* starts;   // ... and the states that sequences of several segments start from: state_out may be state_in
     float* o32;      // ... and the rows of o that the gated norm reads
     int32_t tiles;   // column tiles of a head in the walk
+    int32_t bring;   // the walk has a wave that brings data into the L2
     int32_t split;   // the blocks' matrices: a workgroup per value head
     int32_t seg_blocks;  // blocks of a segment, the last of a sequence may have fewer
     int32_t block_of[TSV_GDN_MAX_SEQ + 1], seg_of[TSV_GDN_MAX_SEQ + 1];  // first block and first segment of every sequence
@@ -103,9 +104,10 @@ __device__ __forceinline__ int sequence_of(const int32_t* starts, int n, int at)
 // One workgroup per (block, key head), wave w owning rows 16 w ..; the products k.k and q.k are made once and shared by the key head's
 // value heads, whose decays make A and P of them.  The inverse: each wave inverts its 16 x 16 diagonal block; then wave j does the blocks
 // under diagonal block j, T_ij = -T_ii sum_l A_il T_lj, on the f32 matrix instruction, whose D layout is its B operand's when the
-// contraction takes rows 4 gq + r in step r.  8192 rows, 16 key and 32 value heads of 128: 76 us for 43 MB read and 174 MB written
-// (2.9 TB/s); the waits of one workgroup, three on a compute unit, bound it.  Few blocks have a workgroup per value head instead
-// (split), each making the products again: 65 rows, 8 heads over 4, 14.4 us against 10.1.
+// contraction takes rows 4 gq + r in step r.  8192 rows, 16 key and 32 value heads of 128: 78 us for 69 MB read and 195 MB written
+// (3.4 TB/s); the waits of one workgroup, three on a compute unit, bound it.  Few blocks have a workgroup per value head instead
+// (split), each making the products again: the whole call with 65 rows, 8 heads over 4, 17.8 us against 21.1; 1024 rows, 32 over 16, 43.7
+// against 45.0; 700 and 800 rows of heads of their own the same.
 // Where P's value (i, j) lies in LDS: rows of 64 values, whose eight 16-byte units take turns from row to row (a column of them, as the
 // fragments are read, would else lie in two banks)
 __device__ __forceinline__ int p_at(int i, int j) { return i * BLK + (((j >> 3) ^ (i & 7)) << 3) + (j & 7); }
@@ -115,7 +117,7 @@ constexpr int blocks_operands = DK > 2 * BLK ? BLK * DK / 8 : 2 * BLK * BLK / 8;
 
 // What a head's decays are in a block.  e^{G_i - G_j} of rows in different row tiles is made of three factors of at most 1: from j to its
 // tile's end, the tiles between, and from the start of i's tile to i; inside a tile it is one exponential of a 64-bit difference.
-// (Two heads' at a time, without what can be made of the others: three workgroups fit a compute unit's LDS to the byte.)
+// (Two heads' at a time, without what can be made of the others: three workgroups fit a compute unit's LDS.)
 struct BlockGates {
     double G[BLK];
     float beta[BLK], from_start[BLK], to_end[BLK];
@@ -346,9 +348,13 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
     GDN_FENCE;                                 \
     __builtin_amdgcn_s_waitcnt(0x0F70);        \
     GDN_FENCE
-// (the wave that brings data into the L2 pays where one workgroup has a compute unit; k_dim 256 needs its registers)
-template <int DK, int NT>
-constexpr int walk_threads = NT == 1 && DK < 256 ? 576 : 512;
+// The wave that brings data into the L2 pays where one workgroup has a compute unit and reads what the last-level cache may not hold any
+// more: of fp16 rows, whose k and q are two terms each, from 128 MB of matrices on (16 / 32 heads of 128: 3000 rows, 105 MB, 116 us with it
+// and 109 without; 5000, 176 MB, 201 and 212; 8192, 288 MB, 355 and 398).  bf16 rows are 2 to 5% faster without it at every length, heads
+// of 64 up to 12%; k_dim 256 has no registers for it.
+template <int DK, bool F16, int NT>
+constexpr int walk_threads = NT == 1 && F16 && DK == 128 ? 576 : 512;
+constexpr int64_t BRING_FROM = 128 << 20;
 
 template <int DK, bool F16, int NT>
 struct Walk {
@@ -385,7 +391,7 @@ struct Walk {
 enum WalkFor { ROWS, NORM, SEGMENTS };
 
 template <int DK, bool F16, int NT, WalkFor FOR>
-__global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape sh, GdnBatch bt, PrefillArgs p) {
+__global__ __launch_bounds__((walk_threads<DK, F16, NT>), 2) void k_gdn_walk(GdnShape sh, GdnBatch bt, PrefillArgs p) {
     typedef Walk<DK, F16, NT> W;
     constexpr bool ENDS = FOR == SEGMENTS;
     constexpr int TR = W::TR, KS = W::KS, SD = W::SD;
@@ -445,7 +451,7 @@ __global__ __launch_bounds__((walk_threads<DK, NT>), 2) void k_gdn_walk(GdnShape
         x.template put<3>(W::D_AT, i >> 1, t, 2 * (i & 1) + (gq >> 1), ed * u);
         if constexpr (!ENDS) x.template put<2>(W::U_AT, i >> 1, t, 2 * (i & 1) + (gq >> 1), u);
     };
-    if (walk_threads<DK, NT> > 512 && w8 == 8) {  // ---- the wave that brings what is four blocks ahead into the XCD's L2, this workgroup's share of it
+    if (walk_threads<DK, F16, NT> > 512 && w8 == 8) {  // ---- the wave that brings what is four blocks ahead into the XCD's L2, this workgroup's share of it
         constexpr int AHEAD = 4, LINES = 3 * KFRAGS<DK, TR> * 8 + TP_UNITS / 8, SHARE = 3;
         const char* kreg = (const char*)(p.kt + (b0 * sh.hk + hk) * (3 * KFRAGS<DK, TR> * 64));
         const int64_t k_step = (int64_t)sh.hk * (3 * KFRAGS<DK, TR> * 1024);
@@ -916,16 +922,16 @@ int launch_walk(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, PrefillA
     if (rc) return rc;
     p.tiles = (sh.dv + (FOR == SEGMENTS ? DK : 0)) / (16 * NT);
     const int heads = p.seg_of[bt.n_seq] * sh.hk;
-    hipLaunchKernelGGL((k_gdn_walk<DK, F16, NT, FOR>), dim3((heads + 7) / 8 * 8 * sh.rep * p.tiles), dim3(walk_threads<DK, NT>), lds, st, sh, bt, p);
+    hipLaunchKernelGGL((k_gdn_walk<DK, F16, NT, FOR>), dim3((heads + 7) / 8 * 8 * sh.rep * p.tiles), dim3(p.bring ? walk_threads<DK, F16, NT> : 512), lds, st, sh, bt, p);
     TSV_HIP(hipGetLastError());
     return TSV_OK;
 }
 
 template <int DK, bool F16, WalkFor FOR>
 int launch_rows(hipStream_t st, const GdnShape& sh, const GdnBatch& bt, PrefillArgs& p) {
-    // Two column tiles a workgroup where that still gives every compute unit one: they share what a block reads (6 sequences, 32 heads of
-    // 128: 72 us against 106); else one, for the shorter way through a block (8192 rows, 32 heads: 185 us against 208).  k_dim 256 has no
-    // registers for two.
+    // Two column tiles a workgroup where that still gives every compute unit one: they share what a block reads (prompts of 1 to 2049 rows, 6
+    // sequences, 32 heads of 128: 157 us in all against 189); else one, for the shorter way through a block (8192 rows, 32 heads: 279 us
+    // against 342).  k_dim 256 has no registers for two.
     if constexpr (DK < 256)
         if (sh.dv % 32 == 0 && (int64_t)p.seg_of[bt.n_seq] * sh.hv * (sh.dv / 32) >= 256) return launch_walk<DK, F16, 2, FOR>(st, sh, bt, p);
     return launch_walk<DK, F16, 1, FOR>(st, sh, bt, p);
@@ -999,6 +1005,7 @@ extern "C" int32_t tsv_gdn_prefill(void* stream, const tsv_gdn_layer* layer, con
     p.ends = (float*)(ws + z.kt + z.tp + z.gates);
     p.starts = (float*)(ws + z.kt + z.tp + z.gates + z.ends);
     p.o32 = io->z ? (float*)(ws + z.kt + z.tp + z.gates + z.ends + z.starts) : nullptr;
+    p.bring = z.kt + z.tp >= BRING_FROM;
     p.seg_blocks = z.seg_blocks;
     p.block_of[0] = p.seg_of[0] = 0;
     for (int s = 0; s < bt.n_seq; s++) {
