@@ -26,6 +26,8 @@ struct GdnShape {
 int gdn_check(const char* who, void* stream, const tsv_gdn_layer* l, const tsv_gdn_batch* b, int max_rows, GdnShape* sh, GdnBatch* kb);
 int gdn_check_layer(const char* who, const tsv_gdn_layer* l, GdnShape* sh);
 int gdn_refuse(const char* who, const char* what);
+// The default stream's other handle (hipStreamLegacy) as the runtime's calls take it: hipStreamGetDevice reads through what it is given.
+inline hipStream_t gdn_stream(void* stream) { return (hipStream_t)stream == hipStreamLegacy ? nullptr : (hipStream_t)stream; }
 bool gdn_rows_ok(const void* p, int64_t stride, int64_t width);
 bool gdn_overlap(const void* a, const void* b, size_t bytes);
 

@@ -613,7 +613,7 @@ __global__ __launch_bounds__(THREADS, DK == 256 ? 2 : 4) void k_gdn_step_one(Gdn
         if (p.record) p.record[((size_t)row * sh.hv + h) * dv + col] = u;
     }
     if (p.state_out) {
-float us[NT];
+        float us[NT];
         one_row_spread<DK>(u, us);
 #pragma unroll
         for (int t = 0; t < NT; t++)
@@ -807,11 +807,11 @@ int gdn_check(const char* who, void* stream, const tsv_gdn_layer* l, const tsv_g
     kb->base = b->base;
     kb->parent = b->parent;
     std::memcpy(kb->off, b->offsets, sizeof(int32_t) * (b->n_seq + 1));
-    if (stream) {  // launches go to the current device
+    if (const hipStream_t st = gdn_stream(stream)) {  // launches go to the current device
         int current = 0;
         hipDevice_t of = 0;
         TSV_HIP(hipGetDevice(&current));
-        TSV_HIP(hipStreamGetDevice((hipStream_t)stream, &of));
+        TSV_HIP(hipStreamGetDevice(st, &of));
         if ((int)of != current) return gdn_refuse(who, "the stream belongs to another device than the current one");
     }
     return TSV_OK;
@@ -892,7 +892,7 @@ extern "C" int32_t tsv_gdn_conv(void* stream, const tsv_gdn_layer* layer, const 
     for (int s = 0; s < bt.n_seq; s++) p.tile_of[s + 1] = p.tile_of[s] + (bt.off[s + 1] - bt.off[s] + p.tile_rows - 1) / p.tile_rows;
     const int tiles = p.tile_of[bt.n_seq];
     if (!tiles) return TSV_OK;
-    const hipStream_t st = (hipStream_t)stream;
+    const hipStream_t st = gdn_stream(stream);
     const bool f16 = layer->dtype == TSV_F16;
     if (layer->k_dim == 64) return f16 ? launch_conv<64, true>(st, sh, bt, p, tiles) : launch_conv<64, false>(st, sh, bt, p, tiles);
     if (layer->k_dim == 128) return f16 ? launch_conv<128, true>(st, sh, bt, p, tiles) : launch_conv<128, false>(st, sh, bt, p, tiles);
@@ -941,7 +941,7 @@ extern "C" int32_t tsv_gdn_step(void* stream, const tsv_gdn_layer* layer, const 
     p.max_rows = 1;
     p.inv_pv = (65536 + sh.dv / 8 - 1) / (sh.dv / 8);
     for (int s = 0; s < bt.n_seq; s++) p.max_rows = std::max(p.max_rows, bt.off[s + 1] - bt.off[s]);
-    const hipStream_t st = (hipStream_t)stream;
+    const hipStream_t st = gdn_stream(stream);
     const bool f16 = layer->dtype == TSV_F16, wide = sh.dv > 128;
 #define TSV_GDN_STEP(DK)                                                                                                   \
     (wide ? (f16 ? launch_step<DK, true, 1024>(st, sh, bt, p) : launch_step<DK, false, 1024>(st, sh, bt, p))              \
@@ -983,7 +983,7 @@ extern "C" int32_t tsv_gdn_commit(void* stream, const tsv_gdn_layer* layer, cons
     p.state_out = io->state_out;
     p.state_stride = more ? io->state_stride : 0;
     p.total_rows = bt.off[bt.n_seq];
-    const hipStream_t st = (hipStream_t)stream;
+    const hipStream_t st = gdn_stream(stream);
     if (layer->k_dim == 64) return launch_commit<64>(st, sh, bt, p, io->n_layers);
     if (layer->k_dim == 128) return launch_commit<128>(st, sh, bt, p, io->n_layers);
     return launch_commit<256>(st, sh, bt, p, io->n_layers);

@@ -1012,7 +1012,7 @@ extern "C" int32_t tsv_gdn_prefill(void* stream, const tsv_gdn_layer* layer, con
         p.block_of[s + 1] = p.block_of[s] + (int32_t)blocks_of(bt, s);
         p.seg_of[s + 1] = p.seg_of[s] + (int32_t)std::max<int64_t>(1, (blocks_of(bt, s) + z.seg_blocks - 1) / z.seg_blocks);
     }
-    const hipStream_t st = (hipStream_t)stream;
+    const hipStream_t st = gdn_stream(stream);
     int done;
     if (dk == 64) done = f16 ? launch_prefill<64, true>(st, sh, bt, p, (int)blocks) : launch_prefill<64, false>(st, sh, bt, p, (int)blocks);
     else if (dk == 128) done = f16 ? launch_prefill<128, true>(st, sh, bt, p, (int)blocks) : launch_prefill<128, false>(st, sh, bt, p, (int)blocks);
