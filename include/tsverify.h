@@ -448,10 +448,11 @@ int64_t tsv_max_context(const tsv_ctx* ctx);
 int64_t tsv_vocab(const tsv_ctx* ctx);
 
 /* ---- recurrent layers: the mixer of a gated-delta-rule layer ---------------------------------
- * What a host that verifies drafts for a hybrid target runs in its recurrent layers, beside the attention layers a handle
- * serves (the reference's one batched verify forward is of such a family: crates/runtime/src/families/qwen/batched.rs:92-456,
- * its state folded by rollback_retaining / commit_pending, real_forward_rollback.rs:268-435,501-530).  There is no handle:
- * like tsv_accept_greedy_noalloc these calls take the caller's DEVICE memory and stream, allocate nothing, copy nothing from
+ * What a host that verifies drafts for a hybrid target runs in its recurrent layers between their projections (the reference's one
+ * batched verify forward is of such a family: crates/runtime/src/families/qwen/batched.rs:92-456, its state folded by
+ * rollback_retaining / commit_pending, real_forward_rollback.rs:268-435,501-530).  The mixer is all there is of such a target here: a
+ * handle runs a model of attention layers as a whole, so the host brings the layer loop, the projections, its attention layers and the
+ * head.  There is no handle: like tsv_accept_greedy_noalloc these calls take the caller's DEVICE memory and stream, allocate nothing, copy nothing from
  * the host, wait for nothing and can be captured into a HIP graph (a stream of the caller's own; that of the current device).
  *
  * One head keeps a state S (k_dim x v_dim); a row with unit vectors q, k, a value row v, a decay g <= 0 and beta takes it to
@@ -513,8 +514,12 @@ int32_t tsv_gdn_conv(void* stream, const tsv_gdn_layer* layer, const tsv_gdn_bat
 /* The delta rule over prompts of any length, in blocks of 64 rows: state_out becomes the state behind each sequence's last row.
  * q, k: n_k_heads x k_dim a row, of unit length or shorter (the blocks' solution is built on that); v: n_v_heads x v_dim; g (a
  * value above 0 counts as 0) and beta as tsv_gdn_conv leaves them.  out: n_v_heads x v_dim a row; z NULL: o as it is.  The norm is
- * taken of o in f32, as in tsv_gdn_step.  The workspace (device, 16-byte aligned) belongs to the call until it has run: calls
- * that may overlap in time take one each. */
+ * taken of o in f32, as in tsv_gdn_step.  Rows and states are as far off as 32-bit sums and the rows' one rounding leave them.  The
+ * workspace (device, 16-byte aligned) belongs to the call until it has run: calls that may overlap in time take one each.  Its size is
+ * that of one batch shape, to be asked for each: of every row of a started block 6 n_k_heads k_dim bytes (fp16 twice that), 360 a value
+ * head, and 4 a value of out if the layer has norm weights (32 heads of 128 over 16, bf16: 40 KB a row); and where few heads leave a long
+ * prompt to be walked in segments, the states and matrices of these, so that a smaller batch can need more than a larger one.  A prompt
+ * may come in several calls, state_out the next one's state_in. */
 typedef struct {
     const void *q, *k, *v;
     int64_t q_stride, k_stride, v_stride;

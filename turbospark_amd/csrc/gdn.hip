@@ -130,8 +130,8 @@ __global__ __launch_bounds__(CONV_THREADS) void k_gdn_conv(GdnShape sh, GdnBatch
 //     T = (I + A)^-1,  A_ij = beta_i D_ij k_i.k_j (j a strict ancestor of i),    P_ij = D_ij q_i.k_j (j an ancestor or i)
 // while the others go on to KS = k S, QS = q S (three bf16 products each: 2^-17, see split2).  Then, for all rows at once,
 // u = T beta (v - e^G KS), o = e^G QS + P u, and for final rows S <- e^G_end S + sum_i D_end,i k_i u_i (f32 matrix instructions).
-// With one sequence the chain of loads and three barriers bounds it (32 heads of 128, 5 rows: 9.0 us; 16-row trees of 4 sequences: 12.9
-// us), with many the state's bytes.
+// With one sequence the chain of loads and three barriers bounds it (32 heads of 128, a call among others: 5 rows 8.6 us; 16-row trees of 4
+// sequences 12.6), with many the state's bytes.
 // Operand order of the contraction over k_dim: lane group gq of the 16x16x32 instruction takes elements 4 gq .. + 3 of both
 // 16-wide halves of its 32, so that two neighbouring D tiles of the f32 update are exactly one B operand.
 

@@ -331,17 +331,19 @@ __global__ __launch_bounds__(256, 3) void k_gdn_blocks(GdnShape sh, GdnBatch bt,
 // ---- the walk through a sequence's blocks --------------------------------------------------------------------------------------------
 // One workgroup of eight waves per (sequence, value head, 16 NT value channels).  Waves 0 to 3 take the state from block to block:
 // wave w owns rows 16 w .. of the block and k_dim / 4 rows of the state, which stay in its accumulators; the state and u pass between
-// them through LDS as bf16 terms in operand order, v - e^G kS as the f32 instruction takes it, three barriers a block.  Waves 4 to 7, one beside each of them on a
-// SIMD, make the output rows from the same LDS (q S behind the first barrier, P u behind the third) and hand the others v, transposed,
-// and the decays through LDS: a load or store of any width holds the CU's address unit for 16 cycles, which bounds a block (12 and 9 of
+// them through LDS as bf16 terms in operand order, v - e^G kS as the f32 instruction takes it, three barriers a block.  Waves 4 to 7, one
+// beside each of them on a SIMD, make the output rows from the same LDS (q S behind the first barrier, P u behind the third) and hand the
+// others v, transposed, and the decays through LDS: a load or store of any width holds the CU's address unit for 16 cycles, which bounds a block (12 and 11 of
 // them a wave here), so two-byte ones are taken together.  Everything a block reads is asked for one block ahead, into the registers
 // just used: the scheduling fences keep the compiler from asking earlier, which would take copies and, with them, waits.  The column
 // tiles of a head read the same k, q, T and P: workgroups are numbered so that they share an XCD's L2.
 // Where few heads leave most of the chip idle a sequence is cut into segments.  A block takes every column of the state alike, S -> M S + c
 // with M the same for all, so a first launch (ENDS) walks all segments but the last at once, from nothing with the rows' v and from the
 // unit matrix with v = 0; the walk of segment n then begins with n products M S + c of its own 16 NT columns.
-// 8192 rows of 32 heads of 128, one column tile on each compute unit: 185 us, 1.4 us a block: the three hand-overs through LDS that follow
-// each other, 0.6 of it the address unit's 84 loads and stores.
+// 8192 rows of 32 heads of 128, one column tile on each compute unit: 200 us, 1.6 us a block: the three hand-overs through LDS that follow
+// each other, 0.6 of it the address unit's 92 loads and stores.  235 where o goes out in f32 for the norm (twice the bytes).  Of two
+// column tiles the output's waves make the second's u: T r takes 4 to 16 f32 products a row tile, and a SIMD whose two waves have row tiles
+// w and 3 - w has 20 of the 80 (segments of 32768 rows: 238 us where the state's waves make them all, 219 so).
 #define GDN_FENCE __builtin_amdgcn_sched_barrier(0)
 // all loads have arrived, and the compiler knows: what is under way before a loop would else count in every wait inside it
 #define GDN_ARRIVED                            \
@@ -831,7 +833,7 @@ __global__ __launch_bounds__((walk_threads<DK, F16, NT>), 2) void k_gdn_walk(Gdn
 #undef GDN_ARRIVED
 
 // ---- the gated norm ----------------------------------------------------------------------------------------------------------------------
-// v_dim / 8 of GROUP neighbouring lanes hold a head's row.  Bound by memory: 8192 rows of 32 heads of 128, 268 MB, NORM_US us.
+// v_dim / 8 of GROUP neighbouring lanes hold a head's row.  Bound by memory: 8192 rows of 32 heads of 128, 268 MB, 46 us (5.8 TB/s).
 template <bool F16>
 __global__ __launch_bounds__(256) void k_gdn_norm(GdnShape sh, const float* o, uint16_t* out, int64_t out_stride, const uint16_t* z, int64_t z_stride, uint32_t heads, int group) {
     const uint32_t at = (blockIdx.x * 256 + threadIdx.x) / group, row = at / sh.hv, h = at - row * sh.hv;
