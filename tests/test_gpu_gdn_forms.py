@@ -188,3 +188,31 @@ def test_blocks_brought_into_the_cache_ahead(gated):
     p.io.state_out = p.io.state_in
     ly.gpu.prefill(p.batch, p.io)
     assert np.array_equal(p.out.get(), rows) and np.array_equal(p.din.get(), S)
+
+
+@pytest.mark.parametrize("hk,hv,dk,dv,dtype,lengths", [
+    (2, 8, 64, 128, BF, [1, 2100, 0]),              # segments, then the norm
+    (4, 8, 64, 32, HF, _ragged(6, 32, 140)),        # two column tiles
+])
+def test_captured_calls_of_these_forms_replay(hk, hv, dk, dv, dtype, lengths):
+    """Replayed with other inputs, the program's own calls between: the same bits as without a graph."""
+    rng = np.random.default_rng(17)
+    ly = Layer(rng, hk, hv, dk, dv, 4, dtype)
+    base = [3 * (s % 2) for s in range(len(lengths))]
+    a, b = (Prompt(rng, ly, lengths, base) for _ in range(2))
+    alone = []
+    for p in (a, b):
+        ly.gpu.prefill(p.batch, p.io)
+        alone.append((p.out.get(), p.dout.get()))
+    stream = hip.Stream()
+    graph = hip.CapturedGraph(stream, lambda s: ly.gpu.prefill(a.batch, a.io, s.h))
+    for source in (b, a, b, b):
+        for dst, src in ((a.dq, source.dq), (a.dk_, source.dk_), (a.dv_, source.dv_), (a.dg, source.dg), (a.db, source.db), (a.dz, source.dz), (a.din, source.din)):
+            dst.put(src.a)
+        graph.launch()
+        stream.sync()
+        rows, S = alone[0] if source is a else alone[1]
+        assert np.array_equal(a.out.get(), rows) and np.array_equal(a.dout.get(), S)
+        a.out.put(np.full_like(a.out.a, 0x1234))
+        ly.gpu.prefill(b.batch, b.io)
+        hip.check(hip.rt().hipDeviceSynchronize(), "sync")

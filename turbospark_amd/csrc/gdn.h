@@ -65,7 +65,7 @@ __device__ __forceinline__ void row8_f32(const uint4& u, float* x) {
 
 // x as two bf16 terms: x - hi - lo is at most 2^-18 of x.  Products of two such pairs without the lo * lo part are 2^-16 to 2^-17
 // off at the very most and 2^-19 on average (one term: 2^-9).  Of results that are rounded to 11 bits and fewer that leaves nothing; u and the
-// state of a few-row step are 3e-7 to 1e-6 off by it, where three terms would leave 1e-7 and cost 1.0 us of 8.6.
+// state of a few-row step are 3e-7 to 1e-6 off by it, where three terms would leave 1e-7 and cost 0.5 us of 8.6.
 __device__ __forceinline__ void split2(float x, __bf16& hi, __bf16& lo) {
     hi = (__bf16)x;
     lo = (__bf16)(x - (float)hi);
