@@ -514,12 +514,12 @@ int32_t tsv_gdn_conv(void* stream, const tsv_gdn_layer* layer, const tsv_gdn_bat
 /* The delta rule over prompts of any length, in blocks of 64 rows: state_out becomes the state behind each sequence's last row.
  * q, k: n_k_heads x k_dim a row, of unit length or shorter (the blocks' solution is built on that); v: n_v_heads x v_dim; g (a
  * value above 0 counts as 0) and beta as tsv_gdn_conv leaves them.  out: n_v_heads x v_dim a row; z NULL: o as it is.  The norm is
- * taken of o in f32, as in tsv_gdn_step.  Rows and states are as far off as 32-bit sums and the rows' one rounding leave them.  The
- * workspace (device, 16-byte aligned) belongs to the call until it has run: calls that may overlap in time take one each.  Its size is
- * that of one batch shape, to be asked for each: of every row of a started block 6 n_k_heads k_dim bytes (fp16 twice that), 360 a value
- * head, and 4 a value of out if the layer has norm weights (32 heads of 128 over 16, bf16: 40 KB a row); and where few heads leave a long
- * prompt to be walked in segments, the states and matrices of these, so that a smaller batch can need more than a larger one.  A prompt
- * may come in several calls, state_out the next one's state_in. */
+ * taken of o in f32, as in tsv_gdn_step.  A state is as far off as 32-bit sums leave it, a row by its one rounding and, before that, by
+ * 2^-16 at most of the size of what o is the sum of.  The workspace (device, 16-byte aligned) belongs to the call until it has run: calls
+ * that may overlap in time take one each.  Its size is that of one batch shape, to be asked for each: of every row of a started block
+ * 6 n_k_heads k_dim bytes (fp16 twice that), 360 a value head, and 4 a value of out if the layer has norm weights (32 heads of 128 over
+ * 16, bf16: 40 KB a row); and where few heads leave a long prompt to be walked in segments, the states and matrices of these, so that a
+ * smaller batch can need more than a larger one.  A prompt may come in several calls, state_out the next one's state_in. */
 typedef struct {
     const void *q, *k, *v;
     int64_t q_stride, k_stride, v_stride;
